@@ -10,7 +10,8 @@ model/kernels/csrc/ops.cpp:29-72.)
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Tuple
+from array import array
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -234,6 +235,173 @@ def sample(out: torch.Tensor, logits: torch.Tensor, temperature: Optional[torch.
     lib = library()
     check(lib, lib.sb_sample(_ptr(out), _ptr(logits), _ptr(temperature), _ptr(seeds), _ptr(counters),
                              M, V, _ptr(scratch), _stream()), "sample")
+
+
+def sample_adjusted(out: torch.Tensor, logits: torch.Tensor, temperature: Optional[torch.Tensor] = None,
+                    seeds: Optional[torch.Tensor] = None, counters: Optional[torch.Tensor] = None,
+                    scratch: Optional[torch.Tensor] = None, *, history: Optional[torch.Tensor] = None,
+                    history_rows: Optional[torch.Tensor] = None, prompt_lens: Optional[torch.Tensor] = None,
+                    lengths: Optional[torch.Tensor] = None, penalties: Optional[torch.Tensor] = None,
+                    bias_starts: Optional[torch.Tensor] = None, bias_ids: Optional[torch.Tensor] = None,
+                    bias_values: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None,
+                    mask_rows: Optional[torch.Tensor] = None, adjusted: Optional[torch.Tensor] = None) -> None:
+    """`sample` on adjusted logits.  With c the number of times a token stands in the row's output and "met" whether it
+    stands in its prompt or output:
+
+        l1 = l / repetition if l > 0 else l * repetition     (met tokens; l1 = l for the others)
+        l2 = l1 - frequency * c - presence * (c > 0)
+        l3 = l2 + bias
+        l4 = l3 where the mask allows the token, else -inf
+
+    out[m] is what `sample` gives for l4 (0 for a row in which nothing is left).  Each of the three parts may be absent:
+    * penalties float32 [M, 3] (repetition > 0, presence, frequency) over `history` int32 [rows, width]: row
+      history_rows[m] holds lengths[m] tokens, of which the first prompt_lens[m] are the prompt (int32 [M] each; tokens
+      outside the vocabulary are passed over);
+    * biases of row m: bias_values[i] (float32) on token bias_ids[i] (int32), i from bias_starts[m] to bias_starts[m + 1] - 1
+      (int32 [M + 1]); a token named twice gets both;
+    * `mask` int32 [masks, ceil(V / 32)]: bit t % 32 of word t // 32 allows token t; mask_rows[m] (int32 [M]) is the row's
+      mask, -1 for none.
+    `adjusted` float32 [M, V] receives l4 (it may be `logits`).  A vocabulary of at most 262,144."""
+    if logits.dim() != 2:
+        raise KernelError(f"logits must be [rows, vocabulary], got {tuple(logits.shape)}")
+    M, V = logits.shape
+    _want(logits, "logits", torch.float32)
+    _want(out, "out", torch.int32, (M,))
+    if temperature is not None:
+        if seeds is None or counters is None:
+            raise KernelError("temperature sampling needs seeds and counters")
+        _want(temperature, "temperature", torch.float32, (M,))
+        _want(seeds, "seeds", torch.int32, (M,))
+        _want(counters, "counters", torch.int32, (M,))
+    width = words = 0
+    if history is not None or penalties is not None:
+        if any(t is None for t in (history, history_rows, prompt_lens, lengths, penalties)):
+            raise KernelError("penalties need history, history_rows, prompt_lens, lengths and penalties")
+        if history.dim() != 2 or history.shape[1] < 1:
+            raise KernelError(f"history must be [rows, tokens], got {tuple(history.shape)}")
+        width = history.shape[1]
+        _want(history, "history", torch.int32)
+        _want(history_rows, "history_rows", torch.int32, (M,))
+        _want(prompt_lens, "prompt_lens", torch.int32, (M,))
+        _want(lengths, "lengths", torch.int32, (M,))
+        _want(penalties, "penalties", torch.float32, (M, 3))
+    if bias_starts is not None or bias_ids is not None or bias_values is not None:
+        if any(t is None for t in (bias_starts, bias_ids, bias_values)):
+            raise KernelError("biases need bias_starts, bias_ids and bias_values")
+        _want(bias_starts, "bias_starts", torch.int32, (M + 1,))
+        _want(bias_ids, "bias_ids", torch.int32, (bias_ids.numel(),))
+        _want(bias_values, "bias_values", torch.float32, (bias_ids.numel(),))
+        if bias_ids.numel() == 0:                           # nobody has a bias, and empty tensors have no address
+            bias_starts = bias_ids = bias_values = None
+    if mask is not None or mask_rows is not None:
+        if mask is None or mask_rows is None:
+            raise KernelError("masks need mask and mask_rows")
+        words = -(-V // 32)
+        if mask.dim() != 2 or mask.shape[1] != words:
+            raise KernelError(f"mask must be [masks, {words}], got {tuple(mask.shape)}")
+        _want(mask, "mask", torch.int32)
+        _want(mask_rows, "mask_rows", torch.int32, (M,))
+    if adjusted is not None:
+        _want(adjusted, "adjusted", torch.float32, (M, V))
+    need = sample_scratch_size(M, V)
+    if scratch is None:
+        scratch = torch.zeros(need, dtype=torch.int32, device=logits.device)
+    _want(scratch, "scratch", torch.int32)
+    if scratch.numel() < need:
+        raise KernelError(f"sample scratch has {scratch.numel()} entries, {need} are needed")
+    lib = library()
+    check(lib, lib.sb_sample_adjusted(
+        _ptr(out), _ptr(logits), _ptr(temperature), _ptr(seeds), _ptr(counters), M, V, _ptr(scratch), _ptr(history), width,
+        _ptr(history_rows), _ptr(prompt_lens), _ptr(lengths), _ptr(penalties), _ptr(bias_starts), _ptr(bias_ids),
+        _ptr(bias_values), _ptr(mask), words, _ptr(mask_rows), _ptr(adjusted), _stream()), "sample_adjusted",
+        kernels=1 if M else 0)
+
+
+def copy_pages(k_pools: torch.Tensor, v_pools: torch.Tensor, src: Sequence[int], dst: Sequence[int]) -> None:
+    """Copy page src[i] to page dst[i] in every layer run of a cache group: k_pools [runs, pages, Hkv, BS, D] and v_pools
+    [runs, pages, Hkv, BS, Dv] of one dtype.
+
+    The numbers are the host's (sequences of ints, no tensors on the device): they are checked here and travel with the
+    launch.  A page may be copied to several places; none is written twice, and none is both read and written (a chain of
+    copies is two calls).  Kernels launched later on the stream, whatever they read early, find the copies done."""
+    if k_pools.dim() != 5 or v_pools.dim() != 5 or k_pools.shape[:4] != v_pools.shape[:4]:
+        raise KernelError(f"pools must be [runs, pages, heads, slots, dim], got {tuple(k_pools.shape)} and {tuple(v_pools.shape)}")
+    _want(k_pools, "k_pools")
+    _want(v_pools, "v_pools", k_pools.dtype)
+    if k_pools.device != v_pools.device:
+        raise KernelError("k_pools and v_pools must be on one device")
+    n = len(src)
+    if len(dst) != n:
+        raise KernelError(f"{n} pages to copy and {len(dst)} places")
+    if n == 0:
+        return
+    runs, pages = k_pools.shape[0], k_pools.shape[1]
+    if k_pools.numel() == 0 or v_pools.numel() == 0:
+        raise KernelError("the pools are empty")
+    try:
+        a, b = array("i", src), array("i", dst)
+    except (TypeError, OverflowError) as e:
+        raise KernelError(f"page numbers must be ints of 32 bits: {e}") from None
+    page = k_pools.stride(1) * k_pools.element_size()
+    value_page = v_pools.stride(1) * v_pools.element_size()
+    lib = library()
+    check(lib, lib.sb_copy_pages(_ptr(k_pools), _ptr(v_pools), a.buffer_info()[0], b.buffer_info()[0], n, runs, pages, page,
+                                 value_page, _stream()), "copy_pages", kernels=lib.sb_copy_pages_kernels(n))
+
+
+def attention_shared_scratch_size(members: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int,
+                                  dtype: torch.dtype) -> Tuple[int, int]:
+    """(float32, int32) entries of scratch that `attention_shared` needs for up to so many members; the int32 ones are zero
+    before the first call."""
+    return library().sb_attention_shared_scratch(members, num_heads, num_kv_heads, head_dim), 1
+
+
+def attention_shared(out: torch.Tensor, q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                     block_table: torch.Tensor, token_rows: torch.Tensor, positions: torch.Tensor, members: torch.Tensor,
+                     group_starts: torch.Tensor, shared_lens: torch.Tensor, num_heads: int, scale: float, window: int = 0,
+                     part: Optional[torch.Tensor] = None, counters: Optional[torch.Tensor] = None,
+                     status: Optional[torch.Tensor] = None) -> None:
+    """Paged attention of single decode tokens whose rows share a prefix: what each shared page holds is read once for all
+    tokens of a family.  Arguments up to `positions` as `attention_decode_mma`; token n is at positions[n] >= 0.
+
+    Families: group g is the tokens members[group_starts[g]] .. members[group_starts[g + 1] - 1] (int32; a token at most
+    once), whose block tables name the same pages for their first shared_lens[g] positions (any number of keys; keys past a
+    token's own position are not seen).  A token that shares nothing is a group of its own with length 0.  Tokens in no
+    group are left alone in `out`.  group_starts int32 [groups + 1] starts at 0; empty groups may stand anywhere.
+
+    Scratch: `part` float32 and `counters` int32 of attention_shared_scratch_size() entries, allocated here if None.
+    `status`: int32 word for the bounded waits of the tensor-core kernel, which is not used without it."""
+    N = q.shape[0]
+    if k_pool.dim() != 4:
+        raise KernelError(f"k_pool must be [pages, heads, slots, dim], got {tuple(k_pool.shape)}")
+    _, Hkv, BS, D = k_pool.shape
+    Hq, M, R = num_heads, members.numel(), shared_lens.numel()
+    _code(q.dtype)
+    _want(q, "q", None, (N, Hq * D))
+    _want(out, "out", q.dtype, (N, Hq * D))
+    _want(k_pool, "k_pool", q.dtype)
+    _want(v_pool, "v_pool", q.dtype, k_pool.shape)
+    _want(block_table, "block_table", torch.int32)
+    if block_table.dim() != 2:
+        raise KernelError(f"block_table must be [rows, pages], got {tuple(block_table.shape)}")
+    _want(token_rows, "token_rows", torch.int32, (N,))
+    _want(positions, "positions", torch.int32, (N,))
+    _want(members, "members", torch.int32, (M,))
+    _want(shared_lens, "shared_lens", torch.int32, (R,))
+    _want(group_starts, "group_starts", torch.int32, (R + 1,))
+    if M == 0 or R == 0:
+        return
+    if part is None or counters is None:
+        floats, ints = attention_shared_scratch_size(M, Hq, Hkv, D, BS, q.dtype)
+        part = torch.empty(floats, dtype=torch.float32, device=q.device) if part is None else part
+        counters = torch.zeros(ints, dtype=torch.int32, device=q.device) if counters is None else counters
+    _want(part, "part", torch.float32)
+    _want(counters, "counters", torch.int32)
+    lib = library()
+    check(lib, lib.sb_attention_shared(
+        _ptr(out), _ptr(part), part.numel(), _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(block_table), block_table.shape[1],
+        _ptr(token_rows), _ptr(positions), _ptr(members), M, _ptr(group_starts), _ptr(shared_lens), R, N, Hq, Hkv, D, BS,
+        int(window), float(scale), _code(q.dtype), _stream()), "attention_shared", kernels=2)
 
 
 def gemm_simt(out: torch.Tensor, a: torch.Tensor, w: torch.Tensor, splits: int = 1, w_older: bool = False) -> None:
