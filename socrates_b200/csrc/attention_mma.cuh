@@ -297,12 +297,13 @@ template <int D, int NBQ> struct ColState {
 //   map(score, key position, column block, which of the thread's two columns): what happens to a raw score first
 //   (`scale_log2` = 1 then: mapped scores are in units of log2); NoMap leaves it alone.
 //   between(p), p = 0..3: called between the phases (the caller issues a later tile's copies there).
+//   NBS: column blocks of the state, of which the first NBQ are worked on.
 struct NoMap {
     __device__ __forceinline__ float operator()(float s, int, int, int) const { return s; }
 };
 
-template <int D, int NBQ, typename Between, typename Map = NoMap>
-__device__ __forceinline__ void warp_tile_decode(ColState<D, NBQ>& st, const uint32_t (&qf)[D / 16][4],
+template <int D, int NBQ, typename Between, typename Map = NoMap, int NBS = NBQ>
+__device__ __forceinline__ void warp_tile_decode(ColState<D, NBS>& st, const uint32_t (&qf)[D / 16][4],
                                                  const bf16* ks, const bf16* vs, int kb, int tile_start, int qpos,
                                                  int klo, int khi, float scale_log2, bool masked, Between between,
                                                  const Map& map = Map{}) {

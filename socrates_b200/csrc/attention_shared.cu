@@ -11,6 +11,7 @@
 // G rows) and one part of their keys; parts are joined by a second kernel.
 #include <math.h>
 
+#include "attention_shared.h"
 #include "common.cuh"
 
 using namespace sb;
@@ -275,30 +276,50 @@ int sm_count() {
 
 }  // namespace
 
-// Floats of scratch for up to M members.
-extern "C" long long sb_attention_shared_scratch(int M, int Hq, int Hkv, int D) {
-    if (M <= 0 || Hkv <= 0 || Hq < Hkv || D <= 0) return 0;
-    long long most = 0;
+// Scratch of a call with up to M members in up to M families, in entries: float32, and int32.
+extern "C" int sb_attention_shared_scratch(int M, int Hq, int Hkv, int D, int page_size, int dtype, long long* floats, long long* ints) {
+    SB_REQUIRE(Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && D > 0 && M > 0, "attention_shared: %d members, %d query heads on %d KV heads of %d",
+               M, Hq, Hkv, D);
+    long long most = 0, whole = 1;
     for (int m = 1; m <= M; ++m) {                           // fewer members are cut into more parts
         int NP, NS;
         rows_parts(m, Hq, Hkv, sm_count(), &NP, &NS);
         const long long need = (long long)m * Hq * (NP + NS) * (D + 2);
         most = need > most ? need : most;
     }
-    return most;
+    if (dtype == SB_BF16) {
+        for (int m = 1; m <= M && sb::shared_stream_supports(m, 1, Hq, Hkv, D, page_size); ++m) {
+            long long f, i;                                  // most families: one a member
+            sb::shared_stream_scratch(m, m, Hq, Hkv, D, sm_count(), &f, &i);
+            most = f > most ? f : most;
+            whole = i > whole ? i : whole;
+        }
+    }
+    *floats = most;
+    *ints = whole;
+    return 0;
 }
 
-extern "C" int sb_attention_shared(void* out, float* part, long long part_floats, const void* q, const void* k_pool,
-                                   const void* v_pool, const int* block_table, int table_width, const int* token_rows,
-                                   const int* positions, const int* members, int M, const int* group_starts,
-                                   const int* shared_lens, int R, int N, int Hq, int Hkv, int D, int page_size, int window,
-                                   float scale, int dtype, cudaStream_t stream) {
+extern "C" int sb_attention_shared(void* out, float* part, long long part_floats, int* lists, long long lists_ints, const void* q,
+                                   const void* k_pool, const void* v_pool, const int* block_table, int table_width,
+                                   const int* token_rows, const int* positions, const int* members, int M,
+                                   const int* group_starts, const int* shared_lens, int R, int N, int Hq, int Hkv, int D,
+                                   int page_size, int window, float scale, int dtype, cudaStream_t stream) {
     SB_REQUIRE(Hkv > 0 && Hq > 0 && Hq % Hkv == 0, "attention_shared: %d query heads on %d KV heads", Hq, Hkv);
     SB_REQUIRE(D % 16 == 0 && D >= 16 && D <= 256, "attention_shared: head_dim %d", D);
     SB_REQUIRE(page_size > 0 && table_width > 0 && window >= 0, "attention_shared: pages of %d, table of %d, window of %d",
                page_size, table_width, window);
-    SB_REQUIRE(N > 0 && M > 0 && M <= N && R > 0 && M <= 65535, "attention_shared: %d members of %d tokens in %d groups", M, N, R);
+    SB_REQUIRE(N > 0 && M > 0 && M <= N && R > 0 && R <= N && M <= 65535, "attention_shared: %d members of %d tokens in %d groups", M, N, R);
     SB_REQUIRE(dtype == SB_F32 || dtype == SB_BF16, "attention_shared: element type %d", dtype);
+    if (dtype == SB_BF16 && sb::shared_stream_supports(M, R, Hq, Hkv, D, page_size)) {
+        long long floats, ints;
+        sb::shared_stream_scratch(M, R, Hq, Hkv, D, sm_count(), &floats, &ints);
+        SB_REQUIRE(part != nullptr && part_floats >= floats && lists != nullptr && lists_ints >= ints, "attention_shared: scratch is too small");
+        const sb::SharedLists l{block_table, token_rows, positions, members, group_starts, shared_lens, table_width, M, R};
+        const int rc = sb::shared_stream(out, part, lists, q, k_pool, v_pool, l, Hq, Hkv, D, page_size, window, scale, sm_count(), stream);
+        if (rc != 0) return rc;
+        SB_LAUNCH_CHECK();
+    }
     const Shared a{block_table, token_rows, positions, members, group_starts, shared_lens, table_width, M, R, Hq, Hkv, D,
                    page_size, window};
     int NP, NS;

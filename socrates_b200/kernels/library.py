@@ -40,7 +40,8 @@ _SIGNATURES = {
     "sb_sample_adjusted": [P, P, P, P, P, I, I, P, P, I, P, P, P, P, P, P, P, P, I, P, P, P],
     "sb_copy_pages": [P, P, P, P, I, I, I, LL, LL, P],
     "sb_copy_pages_kernels": [I],
-    "sb_attention_shared": [P, P, LL, P, P, P, P, I, P, P, P, I, P, P, I, I, I, I, I, I, I, F, I, P],
+    "sb_attention_shared_scratch": [I, I, I, I, I, I, P, P],
+    "sb_attention_shared": [P, P, LL, P, LL, P, P, P, P, I, P, P, P, I, P, P, I, I, I, I, I, I, I, F, I, P],
     "sb_gemm_simt": [P, P, P, I, I, I, I, I, I, I, I, P],
     "sb_attention_simt": [P, P, P, P, P, P, P, I, P, P, I, I, I, I, I, I, F, I, I, P],
     "sb_gemm_tcgen05": [P, P, P, I, I, I, I, P, P, I, I, P, LL, P],
@@ -118,9 +119,6 @@ def declare(lib: ctypes.CDLL, signatures: dict) -> None:
     if hasattr(lib, "sb_selective_scan_scratch"):
         lib.sb_selective_scan_scratch.argtypes = [c_int, c_int, c_int, c_int]
         lib.sb_selective_scan_scratch.restype = c_longlong
-    if hasattr(lib, "sb_attention_shared_scratch"):
-        lib.sb_attention_shared_scratch.argtypes = [c_int, c_int, c_int, c_int]
-        lib.sb_attention_shared_scratch.restype = c_longlong
     lib.sb_last_error.argtypes = []
     lib.sb_last_error.restype = c_char_p
 

@@ -351,15 +351,19 @@ def copy_pages(k_pools: torch.Tensor, v_pools: torch.Tensor, src: Sequence[int],
 
 def attention_shared_scratch_size(members: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int,
                                   dtype: torch.dtype) -> Tuple[int, int]:
-    """(float32, int32) entries of scratch that `attention_shared` needs for up to so many members; the int32 ones are zero
-    before the first call."""
-    return library().sb_attention_shared_scratch(members, num_heads, num_kv_heads, head_dim), 1
+    """(float32, int32) entries of scratch that `attention_shared` needs for up to so many members, in at most as many
+    groups."""
+    floats, ints = ctypes.c_longlong(), ctypes.c_longlong()
+    lib = library()
+    check(lib, lib.sb_attention_shared_scratch(members, num_heads, num_kv_heads, head_dim, page_size, _code(dtype),
+                                               ctypes.byref(floats), ctypes.byref(ints)), "attention_shared_scratch_size", kernels=0)
+    return floats.value, ints.value
 
 
 def attention_shared(out: torch.Tensor, q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
                      block_table: torch.Tensor, token_rows: torch.Tensor, positions: torch.Tensor, members: torch.Tensor,
                      group_starts: torch.Tensor, shared_lens: torch.Tensor, num_heads: int, scale: float, window: int = 0,
-                     part: Optional[torch.Tensor] = None, counters: Optional[torch.Tensor] = None,
+                     part: Optional[torch.Tensor] = None, lists: Optional[torch.Tensor] = None,
                      status: Optional[torch.Tensor] = None) -> None:
     """Paged attention of single decode tokens whose rows share a prefix: what each shared page holds is read once for all
     tokens of a family.  Arguments up to `positions` as `attention_decode_mma`; token n is at positions[n] >= 0.
@@ -369,7 +373,7 @@ def attention_shared(out: torch.Tensor, q: torch.Tensor, k_pool: torch.Tensor, v
     token's own position are not seen).  A token that shares nothing is a group of its own with length 0.  Tokens in no
     group are left alone in `out`.  group_starts int32 [groups + 1] starts at 0; empty groups may stand anywhere.
 
-    Scratch: `part` float32 and `counters` int32 of attention_shared_scratch_size() entries, allocated here if None.
+    Scratch: `part` float32 and `lists` int32 of attention_shared_scratch_size() entries, allocated here if None.
     `status`: int32 word for the bounded waits of the tensor-core kernel, which is not used without it."""
     N = q.shape[0]
     if k_pool.dim() != 4:
@@ -391,16 +395,16 @@ def attention_shared(out: torch.Tensor, q: torch.Tensor, k_pool: torch.Tensor, v
     _want(group_starts, "group_starts", torch.int32, (R + 1,))
     if M == 0 or R == 0:
         return
-    if part is None or counters is None:
+    if part is None or lists is None:
         floats, ints = attention_shared_scratch_size(M, Hq, Hkv, D, BS, q.dtype)
         part = torch.empty(floats, dtype=torch.float32, device=q.device) if part is None else part
-        counters = torch.zeros(ints, dtype=torch.int32, device=q.device) if counters is None else counters
+        lists = torch.empty(ints, dtype=torch.int32, device=q.device) if lists is None else lists
     _want(part, "part", torch.float32)
-    _want(counters, "counters", torch.int32)
+    _want(lists, "lists", torch.int32)
     lib = library()
     check(lib, lib.sb_attention_shared(
-        _ptr(out), _ptr(part), part.numel(), _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(block_table), block_table.shape[1],
-        _ptr(token_rows), _ptr(positions), _ptr(members), M, _ptr(group_starts), _ptr(shared_lens), R, N, Hq, Hkv, D, BS,
+        _ptr(out), _ptr(part), part.numel(), _ptr(lists), lists.numel(), _ptr(q), _ptr(k_pool), _ptr(v_pool),
+        _ptr(block_table), block_table.shape[1], _ptr(token_rows), _ptr(positions), _ptr(members), M, _ptr(group_starts), _ptr(shared_lens), R, N, Hq, Hkv, D, BS,
         int(window), float(scale), _code(q.dtype), _stream()), "attention_shared", kernels=2)
 
 

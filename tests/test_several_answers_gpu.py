@@ -262,13 +262,13 @@ def test_attention_shared_replayed_with_other_families(dtype):
     first.run()
     members, starts, lens = first.lists
     floats, counts = ops.attention_shared_scratch_size(6, 32, 8, 128, PAGE, dtype)
-    part, counters = torch.empty(floats, device="cuda"), torch.zeros(counts, dtype=torch.int32, device="cuda")
+    part, lists = torch.empty(floats, device="cuda"), torch.zeros(counts, dtype=torch.int32, device="cuda")
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
     outs = [torch.zeros(6, 32 * 128, dtype=dtype, device="cuda") for _ in range(2)]
     graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
     for graph, out in zip(graphs, outs):
         with torch.cuda.graph(graph):
-            ops.attention_shared(out, *first.device, *first.lists, 32, 128 ** -0.5, 0, part, counters, status)
+            ops.attention_shared(out, *first.device, *first.lists, 32, 128 ** -0.5, 0, part, lists, status)
     want = first.want()
     for graph, out in zip(graphs, outs):
         graph.replay()
@@ -298,7 +298,7 @@ def test_attention_shared_refusals():
                 dict(group_starts=starts[:1]), dict(num_heads=7), dict(window=-1), dict(members=ints([0, 1, 0])),
                 dict(k_pool=k.half(), v_pool=v.half(), q=q.half(), out=out.half()), dict(token_rows=rows[:1]),
                 dict(part=torch.empty(8, device="cuda")), dict(k_pool=k.cpu()), dict(block_table=table[0]),
-                dict(part=torch.empty(floats, device="cuda"), counters=torch.zeros(9, device="cuda"))):
+                dict(part=torch.empty(floats, device="cuda"), lists=torch.zeros(9, device="cuda"))):
         with pytest.raises(KernelError):
             ops.attention_shared(**{**good, **bad})
     wide = torch.zeros(2, 2 * 264, dtype=torch.bfloat16, device="cuda")
