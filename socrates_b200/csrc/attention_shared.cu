@@ -290,7 +290,7 @@ extern "C" int sb_attention_shared_scratch(int M, int Hq, int Hkv, int D, int pa
     if (dtype == SB_BF16) {
         for (int m = 1; m <= M && sb::shared_stream_supports(m, 1, Hq, Hkv, D, page_size); ++m) {
             long long f, i;                                  // most families: one a member
-            sb::shared_stream_scratch(m, m, Hq, Hkv, D, sm_count(), &f, &i);
+            sb::shared_stream_scratch(m, m, Hq, Hkv, D, page_size, sm_count(), &f, &i);
             most = f > most ? f : most;
             whole = i > whole ? i : whole;
         }
@@ -300,23 +300,35 @@ extern "C" int sb_attention_shared_scratch(int M, int Hq, int Hkv, int D, int pa
     return 0;
 }
 
+// Whether a bfloat16 call launches the kernel for large families too (three kernels instead of two).
+extern "C" int sb_attention_shared_kernels(int M, int R, int Hq, int Hkv, int D, int page_size, int num_pages, int with_status) {
+    return Hkv > 0 && with_status && sb::shared_stream_supports(M, R, Hq, Hkv, D, page_size) &&
+                   sb::shared_tc_supports(M, R, Hq, Hkv, D, page_size, num_pages)
+               ? 3 : 2;
+}
+
 extern "C" int sb_attention_shared(void* out, float* part, long long part_floats, int* lists, long long lists_ints, const void* q,
-                                   const void* k_pool, const void* v_pool, const int* block_table, int table_width,
-                                   const int* token_rows, const int* positions, const int* members, int M,
+                                   const void* k_pool, const void* v_pool, int num_pages, const int* block_table,
+                                   int table_width, const int* token_rows, const int* positions, const int* members, int M,
                                    const int* group_starts, const int* shared_lens, int R, int N, int Hq, int Hkv, int D,
-                                   int page_size, int window, float scale, int dtype, cudaStream_t stream) {
+                                   int page_size, int window, float scale, int dtype, int* status,
+                                   cudaStream_t stream) {
     SB_REQUIRE(Hkv > 0 && Hq > 0 && Hq % Hkv == 0, "attention_shared: %d query heads on %d KV heads", Hq, Hkv);
     SB_REQUIRE(D % 16 == 0 && D >= 16 && D <= 256, "attention_shared: head_dim %d", D);
     SB_REQUIRE(page_size > 0 && table_width > 0 && window >= 0, "attention_shared: pages of %d, table of %d, window of %d",
                page_size, table_width, window);
     SB_REQUIRE(N > 0 && M > 0 && M <= N && R > 0 && R <= N && M <= 65535, "attention_shared: %d members of %d tokens in %d groups", M, N, R);
     SB_REQUIRE(dtype == SB_F32 || dtype == SB_BF16, "attention_shared: element type %d", dtype);
+    const uintptr_t all = reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_pool) |
+                          reinterpret_cast<uintptr_t>(v_pool) | reinterpret_cast<uintptr_t>(part) | reinterpret_cast<uintptr_t>(lists);
+    SB_REQUIRE(all % 16 == 0, "attention_shared: out, q, the pools and the scratch must start on 16 bytes");
     if (dtype == SB_BF16 && sb::shared_stream_supports(M, R, Hq, Hkv, D, page_size)) {
         long long floats, ints;
-        sb::shared_stream_scratch(M, R, Hq, Hkv, D, sm_count(), &floats, &ints);
+        sb::shared_stream_scratch(M, R, Hq, Hkv, D, page_size, sm_count(), &floats, &ints);
         SB_REQUIRE(part != nullptr && part_floats >= floats && lists != nullptr && lists_ints >= ints, "attention_shared: scratch is too small");
         const sb::SharedLists l{block_table, token_rows, positions, members, group_starts, shared_lens, table_width, M, R};
-        const int rc = sb::shared_stream(out, part, lists, q, k_pool, v_pool, l, Hq, Hkv, D, page_size, window, scale, sm_count(), stream);
+        const int rc = sb::shared_stream(out, part, lists, q, k_pool, v_pool, l, Hq, Hkv, D, page_size, num_pages,
+                                         window, scale, sm_count(), status, stream);
         if (rc != 0) return rc;
         SB_LAUNCH_CHECK();
     }

@@ -5,10 +5,11 @@
 // a family's shared keys 16 of its tokens x G rows at a time, so both kinds of work are the same walk.
 //
 // An item is one set of rows with the keys that all of them meet: first the families' units of 16 rows, then the tokens.
-// The 64-key tiles of all items are laid end to end (per KV head) and dealt to the GPU's blocks in equal shares, as in
-// attention_balanced.cu; the cut is made on the device, so a recorded graph follows the lists.  Every item leaves partial
-// results (max, sum, O): one if it lies in one share, one per share otherwise.  A second kernel joins a token's own
-// and its unit's partial results in key order: no atomics, the same bits every time.
+// The 64-key tiles of all items are laid end to end (per KV head) and cut into equal chunks: one a block where there is
+// little to do, else up to four, of which the blocks claim one after the other (a block that starts late, behind the kernel for
+// large families, takes fewer).  The cut is made on the device, so a recorded graph follows the lists.  Every item leaves
+// partial results (max, sum, O): one if it lies in one chunk, one per chunk otherwise.  A second kernel joins a token's
+// own and its unit's partial results in key order: the same bits every time, whoever took a chunk.
 #include <math.h>
 
 #include "attention_mma.cuh"
@@ -18,11 +19,13 @@ namespace {
 
 constexpr int NW = 4;                    // warps of a block; a tile holds 16 keys for each
 constexpr int STAGES = 3;
-constexpr int AHEAD = 7;                 // tiles that page numbers are read ahead (their copies go out STAGES - 1 ahead)
+constexpr int AHEAD = 3;                 // tiles that page numbers are read ahead (their copies go out STAGES - 1 ahead)
+constexpr int CHUNK = AHEAD + 3;         // tiles of a claimed chunk at least
 constexpr int PAGE_SLOTS = 8;            // tiles whose page numbers are held: more than AHEAD, a power of two
 constexpr int TILE_PAGES = 4;            // pages of 16 keys and more
 constexpr int RQ = 16;                   // rows of an item: two column blocks
 constexpr int SMEM_MOST = 220 * 1024, TWO_AN_SM = 112 * 1024;      // dynamic shared memory of a block
+constexpr int MAX_KV_HEADS = 256;
 constexpr int MAX_MEMBERS = 512;         // (their lists live in shared memory)
 
 // Units of 16 rows that the families of M members can have.
@@ -30,12 +33,14 @@ __host__ __device__ inline int most_units(int M, int R, int G) { return M * G / 
 
 struct StreamArgs {
     float *whole_o, *whole_ml;           // [Hkv][items][16][D] and [Hkv][items][16][2]
-    float *piece_o, *piece_ml;           // [Hkv][W][2][16][D] and [Hkv][W][2][16][2]
-    int* items;                          // for the joining kernel: tiles, units, [items + 1] tiles before each, [M] places
+    float *piece_o, *piece_ml;           // [Hkv][4 W][2][16][D] and [Hkv][4 W][2][16][2]
+    int* counters;                       // [Hkv] chunks claimed, zero before and after
+    int* items;                          // for the joining kernel: eight entries a member (see sb::TcPart), -2 first: not served
     const bf16 *q, *k_pool, *v_pool;
     const int *block_table, *token_rows, *positions, *members, *group_starts, *shared_lens;
-    int table_width, M, R, Hq, Hkv, BS, window, W;
+    int table_width, M, R, Hq, Hkv, BS, window, W, num_sms;
     float scale_log2;
+    sb::TcPart tc;                       // items: the large families' shared keys are the kernel's before this one, else null
 };
 
 __device__ __forceinline__ int first_seen(int pos, int window) { return window > 0 && pos + 1 > window ? pos + 1 - window : 0; }
@@ -46,7 +51,7 @@ struct Lists {
     int *starts, *uoff;                  // [R + 1]: members and units before each family
     int *unit, *unit_lo, *unit_hi;       // [units]: first flat row x 32 + rows; keys
     int* pre;                            // [items + 1]: tiles before each item
-    int U, G, window;
+    int U, I, G, window;
     __device__ __forceinline__ int row0(int i) const { return i < U ? unit[i] >> 5 : (i - U) * G; }
     __device__ __forceinline__ int rows(int i) const { return i < U ? unit[i] & 31 : G; }
     __device__ __forceinline__ int lo(int i) const { return i < U ? unit_lo[i] : own_lo[i - U]; }
@@ -60,7 +65,15 @@ struct Cursor {
     int i, begin, end, lo, hi, first;    // first: the tile index inside the row of flat tile 0
     const int* table;
     __device__ __forceinline__ void seek(int x, const Lists& it, const StreamArgs& a) {
-        while (x >= it.pre[i + 1]) ++i;
+        if (x >= it.pre[i + 1]) ++i;                         // the next one, or (after a jump, or behind empty items) a later one
+        if (x >= it.pre[i + 1]) {
+            int top = it.I - 1;
+            while (i < top) {
+                const int mid = (i + top) / 2;
+                if (x >= it.pre[mid + 1]) i = mid + 1;
+                else top = mid;
+            }
+        }
         begin = it.pre[i];
         end = it.pre[i + 1];
         lo = it.lo(i);
@@ -70,6 +83,15 @@ struct Cursor {
     }
     __device__ __forceinline__ int tile_start(int x) const { return (first + x) * KT; }
 };
+
+// The cut for W blocks.  Few tiles: equal chunks, one a block.  More: a block's own chunk is three fifths of an equal share, and
+// the rest goes in chunks of five tiles and more to whoever is done.  (Equal shares alone: a block that starts 20 us late, behind
+// the kernel for large families, ends 20 us late.)
+__device__ __forceinline__ sb::Cut cut_of(int T, int W) {
+    if (T < 15 * W) return sb::Cut{T, max(1, min(W, T)), T, 0};
+    const int T1 = T / 5 * 3;
+    return sb::Cut{T, W, T1, min(3 * W, (T - T1) / CHUNK)};
+}
 
 // Running sum over `n` values in shared memory, v[0] = 0 .. v[n]: v[i + 1] holds the i-th value when it is called.
 __device__ __forceinline__ void running_sum(int* v, int n, int* scan) {
@@ -102,7 +124,10 @@ template <int D>
 __global__ void __launch_bounds__(32 * NW, 2) shared_stream_kernel(const StreamArgs a) {
     sb::pdl_launch_dependents();
     // Before pdl_wait(): the lists, positions, block table (host copies) and keys and values below a row's newest position
-    // (earlier steps).
+    // (earlier steps).  Behind the kernel for large families, which lets this one in when its own wait has returned, queries
+    // and newest keys are complete too (and the partial results of an earlier call are read): this one then runs beside it
+    // and waits for it at its end, for the joining kernel's sake.
+    const bool large = a.tc.items != nullptr;
     constexpr int NTHR = 32 * NW;
     constexpr int STAGE = 2 * KT * D;                       // elements of a stage: keys, then values
     extern __shared__ __align__(128) uint8_t smem[];
@@ -124,7 +149,7 @@ __global__ void __launch_bounds__(32 * NW, 2) shared_stream_kernel(const StreamA
     it.unit_hi = it.unit_lo + units;
     it.pre = it.unit_hi + units;
     __shared__ float w_m[NW][16], w_l[NW][16];
-    __shared__ int s_scan[NW], s_item0;
+    __shared__ int s_scan[NW], s_item0, s_next;
 
     const int bs_log2 = 31 - __clz(a.BS);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -134,7 +159,8 @@ __global__ void __launch_bounds__(32 * NW, 2) shared_stream_kernel(const StreamA
     for (int i = tid; i < a.R; i += NTHR) {
         const int s0 = a.group_starts[i], n = a.group_starts[i + 1] - s0;
         it.starts[i] = s0;
-        it.uoff[i + 1] = a.shared_lens[i] > 0 ? (n * G + RQ - 1) / RQ : 0;
+        const int shared = a.shared_lens[i];
+        it.uoff[i + 1] = shared > 0 && !(large && sb::tc_family(n, G, shared)) ? (n * G + RQ - 1) / RQ : 0;
     }
     if (tid == 0) it.starts[a.R] = a.group_starts[a.R];
     for (int i = tid; i < a.M; i += NTHR) {
@@ -145,7 +171,7 @@ __global__ void __launch_bounds__(32 * NW, 2) shared_stream_kernel(const StreamA
     }
     __syncthreads();
     running_sum(it.uoff, a.R, s_scan);
-    const int U = it.U = it.uoff[a.R], served = min(a.M, it.starts[a.R]), I = U + served;
+    const int U = it.U = it.uoff[a.R], served = min(a.M, it.starts[a.R]), I = it.I = U + served;
     auto family_of = [&](const int* begin, int x) {         // the last one that begins at x or before
         int r = 0, top = a.R - 1;
         while (r < top) {
@@ -176,40 +202,45 @@ __global__ void __launch_bounds__(32 * NW, 2) shared_stream_kernel(const StreamA
     __syncthreads();
     running_sum(it.pre, I, s_scan);
     const int T = it.pre[I];
-    const int W = max(1, min(a.W, T));
+    const sb::Cut cut = cut_of(T, a.W);
+    const int C = cut.pieces();
     if (blockIdx.x == 0) {
-        // the previous call's joining kernel may still read this
-        sb::pdl_wait();
-        int* pre = a.items + 2;
-        int* place = pre + most + 1;
-        if (tid == 0) { a.items[0] = T; a.items[1] = U; }
-        for (int i = tid; i <= I; i += NTHR) pre[i] = it.pre[i];
-        for (int i = tid; i < a.M; i += NTHR) {             // the flat row of a member's first head among the units' rows
-            int p = -2;
+        if (!large) sb::pdl_wait();                         // the previous call's joining kernel may still read this
+        int4* where = reinterpret_cast<int4*>(a.items);
+        for (int i = tid; i < a.M; i += NTHR) {
+            int4 w = make_int4(i < served ? -1 : -2, 0, 0, 0), v = make_int4(0, 0, 0, it.token[i]);
             if (i < served) {
                 const int r = family_of(it.starts, i);
-                p = it.uoff[r + 1] > it.uoff[r] ? it.uoff[r] * RQ + (i - it.starts[r]) * G : -1;
+                if (it.uoff[r + 1] > it.uoff[r]) {
+                    w.x = it.uoff[r] * RQ + (i - it.starts[r]) * G;
+                    const int u = w.x / RQ;
+                    const int2 first = cut.parts(it.pre[u], it.pre[u + 1]), second = cut.parts(it.pre[u + 1], it.pre[u + 2]);
+                    w.y = first.x; w.z = first.y; w.w = second.x; v.x = second.y;
+                }
+                const int2 own = cut.parts(it.pre[U + i], it.pre[U + i + 1]);
+                v.y = own.x; v.z = own.y;
             }
-            place[i] = p;
+            where[2 * i] = w;
+            where[2 * i + 1] = v;
         }
     }
-    if (slot >= W || T == 0) {
+    if (slot >= cut.first || T == 0) {
         sb::pdl_wait();
         return;
     }
-    const int x0 = (int)((long long)slot * T / W), x1 = (int)((long long)(slot + 1) * T / W);
+    int chunk = slot, x0 = cut.begin(slot), x1 = cut.begin(slot + 1);       // the chunk that is worked on
     for (int i = tid; i < I; i += NTHR)
         if (it.pre[i] <= x0 && x0 < it.pre[i + 1]) s_item0 = i;
     __syncthreads();
 
     const int n_pages = max(1, KT >> bs_log2);              // logical pages a tile touches
-    // Bring the physical page of entry e of tile x to its slot (0 where the item does not reach: such keys are never
+    // Bring the physical page of entry e of tile x, the block's at-th, to its slot (0 where the item does not reach: such keys are never
     // read, see load_kv_tile).  Asynchronous: part of the commit group that is open.
-    auto fetch_page = [&](const Cursor& c, int x, int e) {
+    auto fetch_page = [&](const Cursor& c, int x, int at, int e) {
         const int logical = (c.tile_start(x) >> bs_log2) + e;
         const bool valid = logical <= ((c.hi - 1) >> bs_log2);
         asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;"
-                     ::"r"(smem_u32(pages + ((x - x0) % PAGE_SLOTS) * TILE_PAGES + e)),
+                     ::"r"(smem_u32(pages + (at % PAGE_SLOTS) * TILE_PAGES + e)),
                        "l"(c.table + (valid ? logical : 0)), "r"(valid ? 4 : 0)
                      : "memory");
     };
@@ -219,7 +250,7 @@ __global__ void __launch_bounds__(32 * NW, 2) shared_stream_kernel(const StreamA
             Cursor c;
             c.i = s_item0;
             c.seek(x, it, a);
-            fetch_page(c, x, i % n_pages);
+            fetch_page(c, x, i / n_pages, i % n_pages);
         }
     }
     cp_async_commit();
@@ -246,7 +277,7 @@ __global__ void __launch_bounds__(32 * NW, 2) shared_stream_kernel(const StreamA
     const Cursor c0 = cl;
 #pragma unroll
     for (int late = 0; late < 2; ++late) {
-        if (late) sb::pdl_wait();
+        if (late && !large) sb::pdl_wait();
         cl = c0;
 #pragma unroll
         for (int s = 0; s < STAGES - 1; ++s) {
@@ -264,22 +295,41 @@ __global__ void __launch_bounds__(32 * NW, 2) shared_stream_kernel(const StreamA
 #pragma unroll
     for (int s = 1; s < STAGES - 1; ++s) cp_async_commit();
 
+    // Chunks beyond the blocks' first ones are claimed when AHEAD + 3 tiles of the chunk before are left: no earlier, so that a block
+    // that is slow or late claims less.
+    int claimed = C, next_chunk = C, nx0 = 0, nx1 = 0;
+    // the tile `k` after tile x of this block, or -1
+    auto ahead = [&](int x, int k) {
+        const int y = x + k;
+        return y < x1 ? y : y - x1 < nx1 - nx0 ? nx0 + y - x1 : -1;
+    };
+
     const WholeTileCopy<D, KT, NTHR> copy(ring, ring + KT * D, STAGE, a.k_pool, a.v_pool, bs_log2, a.Hkv, kh);
     ColState<D, 2> st;
     st.init();
     uint32_t qf[D / 16][4];
     int cpos[4], clo[4];                                    // the keys that this thread's columns see
     Cursor cc = c0, ct = c0;                                // of the tile that is computed, and of the page read-ahead
-    int stage = STAGES - 1;                                 // of tile x: (x - x0) % STAGES
-    for (int x = x0; x < x1; ++x) {
+    int stage = STAGES - 1;                                 // of the block's at-th tile: at % STAGES
+    for (int x = x0, at = 0;; ++at) {
         stage = stage == STAGES - 1 ? 0 : stage + 1;
         cp_async_wait<STAGES - 2>();
-        __syncthreads();                                    // tile x is there; everybody is done with tile x - 1
-        const int xt = x + AHEAD, xl = x + STAGES - 1;
-        if (xl < x1 && xl >= cl.end) cl.seek(xl, it, a);
-        if (xt < x1) {
+        __syncthreads();                                    // tile x is there; everybody is done with the tile before
+        if (cut.more > 0) {
+            const int left = x1 - x;
+            if (left == AHEAD + 3 && tid == 0) claimed = cut.first + atomicAdd(a.counters + kh, 1);
+            if (left == AHEAD + 2 && tid == 0) s_next = claimed;
+            if (left == AHEAD + 1) {
+                next_chunk = s_next;
+                nx0 = next_chunk < C ? cut.begin(next_chunk) : 0;
+                nx1 = next_chunk < C ? cut.begin(next_chunk + 1) : 0;
+            }
+        }
+        const int xt = ahead(x, AHEAD), xl = ahead(x, STAGES - 1);
+        if (xl >= cl.end) cl.seek(xl, it, a);
+        if (xt >= 0) {
             if (xt >= ct.end) ct.seek(xt, it, a);
-            if (tid < n_pages) fetch_page(ct, xt, tid);
+            if (tid < n_pages) fetch_page(ct, xt, at + AHEAD, tid);
         }
         if (x >= cc.end) cc.seek(x, it, a);
         const int nr = it.rows(cc.i);
@@ -298,17 +348,17 @@ __global__ void __launch_bounds__(32 * NW, 2) shared_stream_kernel(const StreamA
         }
         // the copies of tile xl: in doses between the phases of tile x, or (a tile at an item's edge) at once
         const int stage_l = stage == 0 ? STAGES - 1 : stage - 1;
-        const int* pg_l = pages + ((xl - x0) % PAGE_SLOTS) * TILE_PAGES;
+        const int* pg_l = pages + ((at + STAGES - 1) % PAGE_SLOTS) * TILE_PAGES;
         const int tl = cl.tile_start(xl);
         bool doses = false;
-        if (xl < x1) {
+        if (xl >= 0) {
             doses = tl >= cl.lo && tl + KT <= cl.hi;
             if (!doses) {
                 bf16* ks = ring + stage_l * STAGE;
                 load_kv_tile<D, KT, NTHR>(ks, ks + KT * D, a.k_pool, a.v_pool, pg_l, tl >> bs_log2, bs_log2, a.Hkv, kh, tl,
                                           cl.lo, cl.hi);
             }
-            if (xl == cl.begin) load_query(cl, stage_l);
+            if (xl == cl.begin || xl == nx0) load_query(cl, stage_l);
         }
         auto between = [&](int part) {
             if (doses) copy.dose(part, stage_l, pg_l - (tl >> bs_log2), tl);
@@ -323,9 +373,13 @@ __global__ void __launch_bounds__(32 * NW, 2) shared_stream_kernel(const StreamA
         if (nr <= 8) warp_tile_decode<D, 1>(st, qf, ks, ks + KT * D, warp * 16, ts, 0, 0, 0, 1.0f, false, between, seen);
         else warp_tile_decode<D, 2>(st, qf, ks, ks + KT * D, warp * 16, ts, 0, 0, 0, 1.0f, false, between, seen);
         cp_async_commit();
-        if (x + 1 != x1 && x + 1 != cc.end) continue;
+        const bool chunk_ends = x + 1 == x1;
+        if (!chunk_ends && x + 1 != cc.end) {
+            ++x;
+            continue;
+        }
 
-        // ---- the item, or this share of it, ends: merge the warps through the stage that was just read
+        // ---- the item, or this chunk of it, ends: merge the warps through the stage that was just read
         __syncthreads();
         float* wo = reinterpret_cast<float*>(ring + stage * STAGE);        // [NW][16][D]: exactly a stage
 #pragma unroll
@@ -350,8 +404,8 @@ __global__ void __launch_bounds__(32 * NW, 2) shared_stream_kernel(const StreamA
         }
         __syncthreads();
         st.init();
-        const bool whole = cc.begin >= x0 && cc.end <= x1;  // the item lies in this share
-        const size_t p = whole ? (size_t)kh * most + cc.i : ((size_t)kh * a.W + slot) * 2 + (cc.begin <= x0 ? 0 : 1);
+        const bool whole = cc.begin >= x0 && cc.end <= x1;  // the item lies in this chunk
+        const size_t p = whole ? (size_t)kh * most + (cc.i < U ? cc.i : units + cc.i - U) : ((size_t)kh * 4 * a.W + chunk) * 2 + (cc.begin <= x0 ? 0 : 1);
         float* to_o = (whole ? a.whole_o : a.piece_o) + p * RQ * D;
         float* to_ml = (whole ? a.whole_ml : a.piece_ml) + p * RQ * 2;
         for (int idx = tid * 4; idx < nr * D; idx += NTHR * 4) {
@@ -372,67 +426,113 @@ __global__ void __launch_bounds__(32 * NW, 2) shared_stream_kernel(const StreamA
             *reinterpret_cast<float4*>(to_o + idx) = o;
             if (idx == row * D) *reinterpret_cast<float2*>(to_ml + 2 * row) = make_float2(m, l);
         }
+        ++x;
+        if (chunk_ends) {
+            if (next_chunk >= C) break;
+            chunk = next_chunk;
+            x = x0 = nx0;
+            x1 = nx1;
+            next_chunk = C;
+            nx0 = nx1 = 0;
+        }
     }
     cp_async_wait<0>();
+    if (large) sb::pdl_wait();
 }
 
-// grid (M, Hkv): the G rows of a token of one KV head from its unit's partial results, then its own, in key order.
+// grid (M, Hkv): the G rows of a token of one KV head from its unit's partial results, then its own, in key order.  The
+// threads of a block are two to JOIN groups, each of which takes every so many-th partial result, so that many loads of a token
+// are in flight; the groups' sums are added in the groups' order.
+constexpr int JOIN = 4;
+
 template <int D>
-__global__ void __launch_bounds__(128) shared_stream_join_kernel(bf16* __restrict__ out, const StreamArgs a) {
+__global__ void __launch_bounds__(128 * JOIN, 3)
+shared_stream_join_kernel(bf16* __restrict__ out, const StreamArgs a, int groups) {
     sb::pdl_launch_dependents();
+    __shared__ float4 s_o[JOIN - 1][128];
+    __shared__ float2 s_ml[JOIN - 1][128];
     sb::pdl_wait();
-    const int i = blockIdx.x, kh = blockIdx.y, G = a.Hq / a.Hkv, most = most_units(a.M, a.R, G) + a.M;
-    const int T = a.items[0], U = a.items[1], W = max(1, min(a.W, T));
-    const int* pre = a.items + 2;
-    const int place = pre[most + 1 + i];
-    if (place == -2) return;
-    const int n = a.members[i];
-    for (int idx = threadIdx.x * 4; idx < G * D; idx += blockDim.x * 4) {
+    const int i = blockIdx.x, kh = blockIdx.y, G = a.Hq / a.Hkv;
+    if (i == 0 && threadIdx.x == 0) a.counters[kh] = 0;
+    const int4 w = reinterpret_cast<const int4*>(a.items)[2 * i], v = reinterpret_cast<const int4*>(a.items)[2 * i + 1];
+    if (w.x == -2) return;
+    int4 tw = make_int4(-1, 0, 0, 0);
+    int tv = 0;
+    if (a.tc.items != nullptr) {
+        tw = reinterpret_cast<const int4*>(a.tc.items)[2 * i];
+        tv = a.tc.items[8 * i + 4];
+    }
+    const int threads = blockDim.x / groups, group = threadIdx.x / threads, t = threadIdx.x - group * threads;
+    for (int base = 0; base < G * D; base += threads * 4) {
+        const int idx = base + t * 4;
+        const bool mine = idx < G * D;
         const int g = idx / D, d = idx - g * D;
         float M = -INFINITY, L = 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        auto add = [&](int item, int row) {
-            const int begin = pre[item], end = pre[item + 1];
-            if (end == begin) return;
-            const int s0 = (int)(((long long)(begin + 1) * W + T - 1) / T) - 1, s1 = (int)(((long long)end * W + T - 1) / T);
-            const bool whole = s1 == s0 + 1;
-            constexpr int AT = 8;                           // partial results in flight
-            for (int s = s0; s < s1; s += AT) {
+        auto take = [&](const float2 ml, const float4 x) {
+            if (ml.y == 0.f) return;
+            const float top = fmaxf(M, ml.x), keep = L != 0.f ? exp2f(M - top) : 0.f, f = exp2f(ml.x - top);
+            M = top;
+            L = L * keep + f * ml.y;
+            o.x = o.x * keep + f * x.x; o.y = o.y * keep + f * x.y; o.z = o.z * keep + f * x.z; o.w = o.w * keep + f * x.w;
+        };
+        // the partial results of row `row` of an item of `rows` rows: `whole` is the place of the only one, `piece` that of the
+        // first of several
+        auto add = [&](int from, int end, size_t whole, size_t piece, int row, int rows, const float* whole_o, const float* whole_ml,
+                       const float* piece_o, const float* piece_ml) {
+            const int s0 = from & 0x7fffffff, n = end - s0;
+            if (n == 1) {
+                if (group == 0)
+                    take(__ldcg(reinterpret_cast<const float2*>(whole_ml + (whole * rows + row) * 2)),
+                         __ldcg(reinterpret_cast<const float4*>(whole_o + (whole * rows + row) * D + d)));
+                return;
+            }
+            constexpr int AT = 4;                           // partial results in flight a thread
+            for (int s = group; s < n; s += AT * groups) {
                 float2 ml[AT];
-                float4 v[AT];
+                float4 x[AT];
 #pragma unroll
                 for (int u = 0; u < AT; ++u) {
+                    const int y = s + u * groups;
                     ml[u] = make_float2(-INFINITY, 0.f);
-                    v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (s + u < s1) {
-                        const size_t p = whole ? (size_t)kh * most + item
-                                               : ((size_t)kh * a.W + s + u) * 2 + (begin <= (int)((long long)(s + u) * T / W) ? 0 : 1);
-                        ml[u] = __ldcg(reinterpret_cast<const float2*>((whole ? a.whole_ml : a.piece_ml) + (p * RQ + row) * 2));
-                        v[u] = __ldcg(reinterpret_cast<const float4*>((whole ? a.whole_o : a.piece_o) + (p * RQ + row) * D + d));
+                    x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (y < n) {
+                        const size_t p = (piece + 2 * (s0 + y) + (y == 0 && from < 0 ? 1 : 0)) * rows + row;
+                        ml[u] = __ldcg(reinterpret_cast<const float2*>(piece_ml + p * 2));
+                        x[u] = __ldcg(reinterpret_cast<const float4*>(piece_o + p * D + d));
                     }
                 }
-                float top = M;
 #pragma unroll
-                for (int u = 0; u < AT; ++u)
-                    if (ml[u].y != 0.f) top = fmaxf(top, ml[u].x);
-                const float keep = L != 0.f ? exp2f(M - top) : 0.f;
-                L *= keep;
-                o.x *= keep; o.y *= keep; o.z *= keep; o.w *= keep;
-#pragma unroll
-                for (int u = 0; u < AT; ++u)
-                    if (ml[u].y != 0.f) {
-                        const float f = exp2f(ml[u].x - top);
-                        L += f * ml[u].y;
-                        o.x += f * v[u].x; o.y += f * v[u].y; o.z += f * v[u].z; o.w += f * v[u].w;
-                    }
-                M = top;
+                for (int u = 0; u < AT; ++u) take(ml[u], x[u]);
             }
         };
-        if (place >= 0) add((place + g) / RQ, (place + g) % RQ);
-        add(U + i, g);
-        __nv_bfloat162* to = reinterpret_cast<__nv_bfloat162*>(out + ((size_t)n * a.Hq + kh * G) * D + idx);
-        to[0] = __floats2bfloat162_rn(o.x / L, o.y / L);
-        to[1] = __floats2bfloat162_rn(o.z / L, o.w / L);
+        if (mine) {
+            const int units = most_units(a.M, a.R, G);
+            const size_t first = (size_t)kh * (units + a.M), pieces = (size_t)kh * 8 * a.W;
+            if (tw.x >= 0) {
+                const int row = tw.x + g, unit = row / sb::TC_ROWS;
+                const bool next = unit > tw.x / sb::TC_ROWS;
+                add(next ? tw.w : tw.y, next ? tv : tw.z, (size_t)kh * sb::tc_units(a.M, a.R, G) + unit, (size_t)kh * 2 * a.tc.W,
+                    row % sb::TC_ROWS, sb::TC_ROWS, a.tc.whole_o, a.tc.whole_ml, a.tc.piece_o, a.tc.piece_ml);
+            } else if (w.x >= 0) {
+                const int row = w.x + g, unit = row / RQ;
+                const bool next = unit > w.x / RQ;
+                add(next ? w.w : w.y, next ? v.x : w.z, first + unit, pieces, row % RQ, RQ, a.whole_o, a.whole_ml, a.piece_o, a.piece_ml);
+            }
+            add(v.y, v.z, first + units + i, pieces, g, RQ, a.whole_o, a.whole_ml, a.piece_o, a.piece_ml);
+        }
+        if (group > 0) {
+            s_ml[group - 1][t] = make_float2(M, L);
+            s_o[group - 1][t] = o;
+        }
+        __syncthreads();
+        if (group == 0 && mine) {
+            for (int j = 0; j < groups - 1; ++j) take(s_ml[j][t], s_o[j][t]);
+            __nv_bfloat162* to = reinterpret_cast<__nv_bfloat162*>(out + ((size_t)v.w * a.Hq + kh * G) * D + idx);
+            to[0] = __floats2bfloat162_rn(o.x / L, o.y / L);
+            to[1] = __floats2bfloat162_rn(o.z / L, o.w / L);
+        }
+        __syncthreads();
     }
 }
 
@@ -440,8 +540,8 @@ int stream_smem(int M, int R, int G, int D) {
     return (STAGES * 2 * KT * D + STAGES * RQ * D) * 2 + PAGE_SLOTS * TILE_PAGES * 4 + list_ints(M, R, most_units(M, R, G)) * 4;
 }
 
-// Shares a KV head's tiles are cut into: as many blocks as the GPU holds at once (two an SM, or one beside long lists).
-int shares_of(int M, int R, int Hq, int Hkv, int D, int num_sms) {
+// Blocks of a KV head: as many as the GPU holds at once (two an SM, or one beside long lists).
+int blocks_of(int M, int R, int Hq, int Hkv, int D, int num_sms) {
     const int w = num_sms * (stream_smem(M, R, Hq / Hkv, D) <= TWO_AN_SM ? 2 : 1) / Hkv;
     return w < 1 ? 1 : w;
 }
@@ -458,7 +558,10 @@ int launch_stream(void* out, StreamArgs a, cudaStream_t stream) {
         configured = true;
     }
     sb::launch(kernel, dim3(a.W * a.Hkv), dim3(32 * NW), smem, stream, a);
-    sb::launch(shared_stream_join_kernel<D>, dim3(a.M, a.Hkv), dim3(G * D >= 512 ? 128 : 64), 0, stream, (bf16*)out, a);
+    // (four groups where all blocks of four fit the GPU at once)
+    const int groups = a.M * a.Hkv <= 3 * a.num_sms ? JOIN : 2;
+    sb::launch(shared_stream_join_kernel<D>, dim3(a.M, a.Hkv), dim3(groups * (G * D >= 512 ? 128 : G * D >= 256 ? 64 : 32)), 0, stream,
+               (bf16*)out, a, groups);
     return 0;
 }
 
@@ -467,35 +570,53 @@ int launch_stream(void* out, StreamArgs a, cudaStream_t stream) {
 namespace sb {
 
 bool shared_stream_supports(int M, int R, int Hq, int Hkv, int D, int page_size) {
-    if (Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq / Hkv > RQ || M <= 0 || M > MAX_MEMBERS || R <= 0) return false;
+    if (Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq / Hkv > RQ || Hkv > MAX_KV_HEADS || M <= 0 || M > MAX_MEMBERS || R <= 0) return false;
     if (!(D == 16 || D == 32 || D == 64 || D == 128)) return false;
     if (page_size < KT / TILE_PAGES || (page_size & (page_size - 1)) != 0) return false;
     return stream_smem(M, R, Hq / Hkv, D) <= SMEM_MOST;
 }
 
-void shared_stream_scratch(int M, int R, int Hq, int Hkv, int D, int num_sms, long long* floats, long long* ints) {
-    const int items = most_units(M, R, Hq / Hkv) + M;
-    // (as many shares as two blocks an SM make, whatever this call's lists leave room for: no less for more members)
-    *floats = ((long long)Hkv * items + 2ll * (2 * num_sms > Hkv ? 2 * num_sms : Hkv)) * RQ * (D + 2);
-    *ints = 2 + items + 1 + M;
+// Entries for at most M members in at most R families; calls with fewer need no more.
+void shared_stream_scratch(int M, int R, int Hq, int Hkv, int D, int page_size, int num_sms, long long* floats, long long* ints) {
+    const int G = Hq / Hkv, items = most_units(M, R, G) + M;
+    const long long blocks = 2ll * num_sms > Hkv ? 2ll * num_sms : Hkv;          // of all KV heads, two an SM
+    *floats = ((long long)Hkv * items + 8 * blocks) * RQ * (D + 2);
+    *ints = MAX_KV_HEADS + 8ll * M;
+    if (shared_tc_supports(M, R, Hq, Hkv, D, page_size, 1)) {
+        *floats += ((long long)Hkv * tc_units(M, R, G) + 2 * (num_sms > Hkv ? num_sms : Hkv)) * TC_ROWS * (D + 2);
+        *ints += 8ll * M;
+    }
 }
 
 int shared_stream(void* out, float* part, int* items, const void* q, const void* k_pool, const void* v_pool,
-                  const SharedLists& l, int Hq, int Hkv, int D, int page_size, int window, float scale, int num_sms,
-                  cudaStream_t stream) {
+                  const SharedLists& l, int Hq, int Hkv, int D, int page_size, long long num_pages, int window, float scale,
+                  int num_sms, int* status, cudaStream_t stream) {
     StreamArgs a{};
-    const int W = shares_of(l.M, l.R, Hq, Hkv, D, num_sms);
-    const long long most = most_units(l.M, l.R, Hq / Hkv) + l.M;
+    const int G = Hq / Hkv, W = blocks_of(l.M, l.R, Hq, Hkv, D, num_sms);
+    const long long most = most_units(l.M, l.R, G) + l.M;
     a.whole_o = part;
     a.whole_ml = a.whole_o + Hkv * most * RQ * D;
     a.piece_o = a.whole_ml + Hkv * most * RQ * 2;
-    a.piece_ml = a.piece_o + 2ll * Hkv * W * RQ * D;
-    a.items = items;
+    a.piece_ml = a.piece_o + 8ll * Hkv * W * RQ * D;
+    a.counters = items;                  // the first entries, whatever the call: no other call's lists lie there
+    a.items = items + MAX_KV_HEADS;
     a.q = (const bf16*)q; a.k_pool = (const bf16*)k_pool; a.v_pool = (const bf16*)v_pool;
     a.block_table = l.block_table; a.token_rows = l.token_rows; a.positions = l.positions;
     a.members = l.members; a.group_starts = l.group_starts; a.shared_lens = l.shared_lens;
     a.table_width = l.table_width; a.M = l.M; a.R = l.R; a.Hq = Hq; a.Hkv = Hkv; a.BS = page_size; a.window = window; a.W = W;
+    a.num_sms = num_sms;
     a.scale_log2 = scale * LOG2E;
+    if (status != nullptr && shared_tc_supports(l.M, l.R, Hq, Hkv, D, page_size, num_pages)) {
+        const long long units = tc_units(l.M, l.R, G);
+        a.tc.W = num_sms > Hkv ? num_sms / Hkv : 1;          // a block an SM: beside it stays room for one of the walk's
+        a.tc.whole_o = a.piece_ml + 8ll * Hkv * W * RQ * 2;
+        a.tc.whole_ml = a.tc.whole_o + Hkv * units * TC_ROWS * D;
+        a.tc.piece_o = a.tc.whole_ml + Hkv * units * TC_ROWS * 2;
+        a.tc.piece_ml = a.tc.piece_o + 2ll * Hkv * a.tc.W * TC_ROWS * D;
+        a.tc.items = a.items + 8ll * l.M;
+        const int rc = shared_tc(a.tc, q, k_pool, v_pool, l, Hq, Hkv, D, page_size, num_pages, window, scale, status, stream);
+        if (rc != 0) return rc;
+    }
     switch (D) {
         case 16: return launch_stream<16>(out, a, stream);
         case 32: return launch_stream<32>(out, a, stream);

@@ -164,8 +164,15 @@ struct Adjust {
 constexpr int SLICE = 8192;          // logits of a block, whose counts and biases are held in shared memory
 
 // sample_kernel with adjusted logits.  A block counts the row's tokens that fall into its slice (integer atomics in shared
-// memory: the order does not matter), so no table as wide as the vocabulary is kept from step to step.
-__global__ void __launch_bounds__(512)
+// memory: the order does not matter), so no table as wide as the vocabulary is kept from step to step.  What bounds it: the
+// logits' bytes and, for rows that draw, two logarithms a logit.  A thread holds its 16 logits in registers, loaded (16 bytes
+// each where rows allow it) before the counts are made; logits of tokens that a mask forbids are not read.
+//
+// A row that draws needs the noise of few logits: with N = 2^23 - (hash >> 9) in [1, 2^23] the noise -log(-log(u)) is at most
+// -log(1 - u) = log(2^23 / (N - 1/2)).  A block first takes the largest of the scores of its threads' largest logits; a logit l
+// can exceed that, F, only where N - 1/2 <= 2^23 e^(l / T - F), and the others are not looked at.
+// 64 rows of 151,936 logits, half of them drawn, tokens of up to 4,096 and 40 biases a row: 60 us a logit at a time, 42 so.
+__global__ void __launch_bounds__(512, 2)
 sample_adjusted_kernel(int* __restrict__ out, const float* __restrict__ logits, const float* __restrict__ temperature,
                        const uint32_t* __restrict__ seeds, const uint32_t* __restrict__ counters, int V, int per,
                        int* __restrict__ scratch, const Adjust a) {
@@ -177,9 +184,49 @@ sample_adjusted_kernel(int* __restrict__ out, const float* __restrict__ logits, 
     __shared__ float s_val[32];
     __shared__ int s_idx[32];
     __shared__ int s_last;
+    constexpr int THREADS = 512, J = SLICE / (4 * THREADS);  // four times four logits a thread
     const int m = blockIdx.x, C = gridDim.y, tid = threadIdx.x;
     const int lane = tid & 31, warp = tid >> 5;
     const float* row = logits + (size_t)m * V;
+    const int begin = min(V, (int)blockIdx.y * per), end = min(V, begin + per);
+    // logit (j, e) of a thread is `at + 2048 j + step e`: neighbours where 16-byte loads are possible
+    const bool wide = V % 4 == 0 && ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(a.adjusted)) & 15) == 0;
+    const int at = begin + (wide ? 4 * tid : tid), step = wide ? 1 : THREADS;
+
+    const int mask_row = a.mask != nullptr ? a.mask_rows[m] : -1;
+    uint32_t may = 0xffffu;                                 // bit 4 j + e: the token is allowed
+    if (mask_row >= 0) {
+        const uint32_t* allowed = a.mask + (size_t)mask_row * a.mask_words;
+        may = 0;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int i = at + 4 * THREADS * j;
+            if (wide) {
+                if (i < end) may |= (allowed[i >> 5] >> (i & 31) & 15u) << (4 * j);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (i + step * e < end) may |= (allowed[(i + step * e) >> 5] >> ((i + step * e) & 31) & 1u) << (4 * j + e);
+            }
+        }
+    }
+    // a place behind the slice holds NaN, which is never the best, one that is not allowed -inf
+    float v[4 * J];
+    const float none = __int_as_float(0x7fffffff);
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        const int i = at + 4 * THREADS * j;
+        float4 x = make_float4(none, none, none, none);
+        if (wide) {
+            if (i < end) x = may >> (4 * j) & 15u ? *reinterpret_cast<const float4*>(row + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+        } else {
+            if (i < end) x.x = row[i];
+            if (i + step < end) x.y = row[i + step];
+            if (i + 2 * step < end) x.z = row[i + 2 * step];
+            if (i + 3 * step < end) x.w = row[i + 3 * step];
+        }
+        v[4 * j] = x.x; v[4 * j + 1] = x.y; v[4 * j + 2] = x.z; v[4 * j + 3] = x.w;
+    }
     const float T = temperature ? temperature[m] : 0.f;
     uint32_t key = 0;
     if (T > 0.f) {
@@ -187,77 +234,162 @@ sample_adjusted_kernel(int* __restrict__ out, const float* __restrict__ logits, 
         key = mix32(key ^ mix32(counters[m] + 0x85EBCA6Bu));
     }
     const float inv_t = T > 0.f ? 1.0f / T : 1.0f;
-    const int begin = min(V, (int)blockIdx.y * per), end = min(V, begin + per), n = end - begin;
 
+    // ---- counts and biases of the slice's tokens
     const bool penal = a.history != nullptr, biased = a.bias_starts != nullptr;
+    if (penal || biased) {
+        const int4 zero = make_int4(0, 0, 0, 0);
+        for (int i = 4 * tid; i < per * (penal + biased); i += 4 * THREADS) *reinterpret_cast<int4*>(count + i) = zero;
+        __syncthreads();
+    }
     float rep = 1.f, presence = 0.f, frequency = 0.f;
-    if (penal)
-        for (int i = tid; i < n; i += blockDim.x) count[i] = 0;
-    if (biased)
-        for (int i = tid; i < n; i += blockDim.x) bias[i] = 0.f;
-    __syncthreads();
+    const int n = end - begin;
     if (penal) {
         rep = a.penalties[3 * m];
         presence = a.penalties[3 * m + 1];
         frequency = a.penalties[3 * m + 2];
         const int* told = a.history + (size_t)a.history_rows[m] * a.history_width;
         const int len = min(a.lengths[m], a.history_width), prompt = a.prompt_lens[m];
-        for (int i = tid; i < len; i += blockDim.x) {
-            const int t = told[i] - begin;
-            if (t < 0 || t >= n) continue;
-            if (i < prompt) atomicOr(&count[t], (int)0x80000000u);
-            else atomicAdd(&count[t], 1);
+        constexpr int AT = 8;                               // loads in flight
+        for (int i0 = tid; i0 < len; i0 += AT * THREADS) {
+            int t[AT];
+#pragma unroll
+            for (int u = 0; u < AT; ++u) t[u] = i0 + u * THREADS < len ? told[i0 + u * THREADS] - begin : -1;
+#pragma unroll
+            for (int u = 0; u < AT; ++u)
+                if (t[u] >= 0 && t[u] < n) {
+                    if (i0 + u * THREADS < prompt) atomicOr(&count[t[u]], (int)0x80000000u);
+                    else atomicAdd(&count[t[u]], 1);
+                }
         }
     }
-    if (biased && warp == 0) {
+    if (biased && warp == THREADS / 32 - 1) {
         // in the order of the list, so that a token named twice gets both in that order
         const int e1 = a.bias_starts[m + 1];
         for (int e0 = a.bias_starts[m]; e0 < e1; e0 += 32) {
             const int t = e0 + lane < e1 ? a.bias_ids[e0 + lane] - begin : -1;
+            const float x = e0 + lane < e1 ? a.bias_values[e0 + lane] : 0.f;
             const bool mine = t >= 0 && t < n;
             const uint32_t same = __match_any_sync(0xffffffffu, mine ? t : -1 - lane);
             const int rank = __popc(same & ((1u << lane) - 1u));
             const int rounds = __reduce_max_sync(0xffffffffu, rank);
             for (int r = 0; r <= rounds; ++r) {
-                if (mine && rank == r) bias[t] += a.bias_values[e0 + lane];
+                if (mine && rank == r) bias[t] += x;
                 __syncwarp();
             }
         }
     }
-    __syncthreads();
+    if (penal || biased) __syncthreads();
 
-    const int mask_row = a.mask != nullptr ? a.mask_rows[m] : -1;
-    const uint32_t* allowed = mask_row >= 0 ? a.mask + (size_t)mask_row * a.mask_words : nullptr;
-    float best = -INFINITY;
-    int best_i = 0x7fffffff;
-    auto adjust = [&](float v, int i) {
-        if (penal) {
-            const int c = count[i - begin];
-            if (c != 0) {
-                v = v > 0.f ? v / rep : v * rep;
-                const int made = c & 0x7fffffff;
-                if (made > 0) v = v - frequency * (float)made - presence;
+    // ---- the adjusted logits
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        const int i = at + 4 * THREADS * j;
+        if (penal && i < end) {
+            int c[4] = {0, 0, 0, 0};
+            if (wide) {
+                const int4 x = *reinterpret_cast<const int4*>(count + i - begin);
+                c[0] = x.x; c[1] = x.y; c[2] = x.z; c[3] = x.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (i + step * e < end) c[e] = count[i + step * e - begin];
+            }
+            if (c[0] | c[1] | c[2] | c[3]) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (c[e] != 0) {
+                        float x = v[4 * j + e];
+                        x = x > 0.f ? x / rep : x * rep;
+                        const int made = c[e] & 0x7fffffff;
+                        v[4 * j + e] = made > 0 ? x - frequency * (float)made - presence : x;
+                    }
             }
         }
-        if (biased) v += bias[i - begin];
-        return v;
-    };
-    auto look = [&](float v, int i) {
-        if (T > 0.f) {
-            const float u = uniform_for(key, (uint32_t)i);
-            v = v * inv_t - logf(-logf(u));
+        if (biased && i < end) {
+            if (wide) {
+                const float4 x = *reinterpret_cast<const float4*>(bias + i - begin);
+                v[4 * j] += x.x; v[4 * j + 1] += x.y; v[4 * j + 2] += x.z; v[4 * j + 3] += x.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (i + step * e < end) v[4 * j + e] += bias[i + step * e - begin];
+            }
         }
-        if (better(v, i, best, best_i)) { best = v; best_i = i; }
-    };
-    for (int i = begin + tid; i < end; i += blockDim.x) {
-        const bool may = allowed == nullptr || (allowed[i >> 5] >> (i & 31)) & 1u;
-        float v = -INFINITY;
-        if (may) {
-            v = adjust(row[i], i);
-            look(v, i);
-        }
-        if (a.adjusted != nullptr) a.adjusted[(size_t)m * V + i] = v;
     }
+    if (mask_row >= 0) {
+#pragma unroll
+        for (int k = 0; k < 4 * J; ++k)
+            if (!(may >> k & 1u) && at + 4 * THREADS * (k / 4) + step * (k % 4) < end) v[k] = -INFINITY;
+    }
+    if (a.adjusted != nullptr) {
+        float* to = a.adjusted + (size_t)m * V;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int i = at + 4 * THREADS * j;
+            if (wide) {
+                if (i < end) *reinterpret_cast<float4*>(to + i) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (i + step * e < end) to[i + step * e] = v[4 * j + e];
+            }
+        }
+    }
+
+    // ---- the best of them.  A thread's places come in the order of their indices, so the first of equal ones stays.
+    float best = -INFINITY;
+    int best_k = -1;
+    if (T > 0.f) {
+        auto score = [&](float x, int k) {                  // as sample_kernel's, operation by operation
+            const float u = uniform_for(key, (uint32_t)(at + 4 * THREADS * (k / 4) + step * (k % 4)));
+            return x * inv_t - logf(-logf(u));
+        };
+        float top = -INFINITY;
+        int top_k = -1;
+#pragma unroll
+        for (int k = 0; k < 4 * J; ++k)
+            if (v[k] > top) { top = v[k]; top_k = k; }
+        float least = top_k >= 0 ? score(top, top_k) : -INFINITY;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) least = fmaxf(least, __shfl_xor_sync(0xffffffffu, least, o));
+        if (lane == 0) s_val[warp] = least;
+        __syncthreads();
+        least = s_val[lane & (THREADS / 32 - 1)];
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) least = fmaxf(least, __shfl_xor_sync(0xffffffffu, least, o));
+        // l / T in units of log2, less F, and 23: the exponent of the largest N.  2e-3 and 2e-6 of a score are far more than the
+        // roundings on both sides.
+        constexpr float LOG2E = 1.4426950408889634f;
+        const float slope = inv_t * LOG2E, offset = 23.0f + 2e-3f + 2e-6f * fabsf(least) - least * LOG2E;
+        uint32_t look = 0;
+#pragma unroll
+        for (int k = 0; k < 4 * J; ++k) {
+            const uint32_t i = (uint32_t)(at + 4 * THREADS * (k / 4) + step * (k % 4));
+            const float N = (float)(8388608u - (mix32((i + 0x165667B1u) ^ key) >> 9));
+            const float exponent = fmaf(v[k], slope, offset);
+            float most;
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(most) : "f"(fmaf(fabsf(exponent), 2e-6f, exponent)));
+            if (!(N - 0.5f > most)) look |= 1u << k;        // NaN and infinities are looked at
+        }
+        while (__any_sync(0xffffffffu, look != 0)) {         // in the order of the places
+            const int k = __ffs(look) - 1;
+            if (k >= 0) {
+                float x = v[0];
+#pragma unroll
+                for (int y = 1; y < 4 * J; ++y) x = k == y ? v[y] : x;
+                x = score(x, k);
+                if (x > best) { best = x; best_k = k; }
+                look &= look - 1;
+            }
+        }
+        __syncthreads();                                    // s_val is written again below
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4 * J; ++k)
+            if (v[k] > best) { best = v[k]; best_k = k; }
+    }
+    int best_i = best_k < 0 ? 0x7fffffff : at + 4 * THREADS * (best_k >> 2) + step * (best_k & 3);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         const float ov = __shfl_xor_sync(0xffffffffu, best, o);
@@ -268,7 +400,6 @@ sample_adjusted_kernel(int* __restrict__ out, const float* __restrict__ logits, 
     __syncthreads();
     merge_slices(out, scratch, m, C, best, best_i, s_val, s_idx, &s_last);
 }
-
 
 }  // namespace
 
@@ -297,14 +428,16 @@ extern "C" int sb_sample(int* out, const float* logits, const float* temperature
 // bias_starts[m] .. bias_starts[m + 1] - 1.  mask: bit t % 32 of word t / 32 of row mask_rows[m] allows token t.  `adjusted`
 // may be `logits`.  Any of the three parts may be absent (null).
 extern "C" int sb_sample_adjusted(int* out, const float* logits, const float* temperature, const uint32_t* seeds,
-                                  const uint32_t* counters, int M, int V, int* scratch, const int* history, int history_width,
+                                  const uint32_t* counters, int M, int V, int* scratch, long long scratch_ints,
+                                  const int* history, int history_width,
                                   const int* history_rows, const int* prompt_lens, const int* lengths, const float* penalties,
                                   const int* bias_starts, const int* bias_ids, const float* bias_values, const void* mask,
                                   int mask_words, const int* mask_rows, float* adjusted, cudaStream_t stream) {
     SB_REQUIRE(M >= 0 && V > 0, "sample_adjusted: bad sizes M=%d V=%d", M, V);
     SB_REQUIRE(temperature == nullptr || (seeds != nullptr && counters != nullptr),
                "sample_adjusted: temperature sampling needs seeds and counters");
-    SB_REQUIRE(scratch != nullptr, "sample_adjusted: scratch is required");
+    SB_REQUIRE(scratch != nullptr && scratch_ints >= (long long)M * (2 * sb_sample_slices(V) + 1),
+               "sample_adjusted: scratch has %lld entries, %lld are needed", scratch_ints, (long long)M * (2 * sb_sample_slices(V) + 1));
     SB_REQUIRE(V <= 32 * SLICE, "sample_adjusted: a vocabulary of %d (at most %d)", V, 32 * SLICE);
     SB_REQUIRE(history == nullptr || (history_width > 0 && history_rows != nullptr && prompt_lens != nullptr &&
                                       lengths != nullptr && penalties != nullptr),

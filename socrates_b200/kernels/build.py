@@ -36,7 +36,8 @@ CORE_SOURCES = ["errors.cu", "run_calls.cu", "elementwise.cu", "sampling.cu", "g
                 "attention_tcgen05.cu", "fold_norm.cu", "short_conv.cu", "retention.cu", "selective_scan.cu",
                 "attention_bias.cu", "delta_rule.cu", "moe_route.cu", "attention_diff.cu", "hyper_norm.cu",
                 "recurrent_gates.cu", "gated_units.cu", "attention_talk.cu", "linear_recurrence.cu",
-                "attention_latent.cu", "copy_pages.cu", "attention_shared.cu", "attention_shared_mma.cu"]
+                "attention_latent.cu", "copy_pages.cu", "attention_shared.cu", "attention_shared_mma.cu",
+                "attention_shared_tc.cu"]
 
 
 class BuildError(RuntimeError):

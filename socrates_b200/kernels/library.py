@@ -37,11 +37,12 @@ _SIGNATURES = {
     "sb_silu_mul": [P, P, I, I, I, I, I, P],
     "sb_sample": [P, P, P, P, P, I, I, P, P],
     "sb_sample_slices": [I],
-    "sb_sample_adjusted": [P, P, P, P, P, I, I, P, P, I, P, P, P, P, P, P, P, P, I, P, P, P],
+    "sb_sample_adjusted": [P, P, P, P, P, I, I, P, LL, P, I, P, P, P, P, P, P, P, P, I, P, P, P],
     "sb_copy_pages": [P, P, P, P, I, I, I, LL, LL, P],
     "sb_copy_pages_kernels": [I],
     "sb_attention_shared_scratch": [I, I, I, I, I, I, P, P],
-    "sb_attention_shared": [P, P, LL, P, LL, P, P, P, P, I, P, P, P, I, P, P, I, I, I, I, I, I, I, F, I, P],
+    "sb_attention_shared_kernels": [I, I, I, I, I, I, I, I],
+    "sb_attention_shared": [P, P, LL, P, LL, P, P, P, I, P, I, P, P, P, I, P, P, I, I, I, I, I, I, I, F, I, P, P],
     "sb_gemm_simt": [P, P, P, I, I, I, I, I, I, I, I, P],
     "sb_attention_simt": [P, P, P, P, P, P, P, I, P, P, I, I, I, I, I, I, F, I, I, P],
     "sb_gemm_tcgen05": [P, P, P, I, I, I, I, P, P, I, I, P, LL, P],

@@ -54,7 +54,19 @@ class stream_scope:
 
 
 def _stream():
-    return _scoped_stream if _scoped_stream is not None else torch.cuda.current_stream().cuda_stream
+    if _scoped_stream is not None:
+        return _scoped_stream
+    # torch.cuda.current_stream() makes a Stream object, which takes 4 us; this is the handle it holds
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+
+
+def _check(device: int, wanted) -> None:
+    """What `_want` checks, for many tensors at the price of a few, and that they are on one device, the current one:
+    `wanted` holds (tensor, name, dtype, shape or None)."""
+    for t, name, dtype, shape in wanted:
+        if t.get_device() != device or t.dtype is not dtype or not t.is_contiguous() or (shape is not None and t.shape != shape):
+            _want(t, name, dtype, shape)
+            raise KernelError(f"{name} is on {t.device}, not on the current device cuda:{device}")
 
 
 def set_dependent_launch(on: bool) -> None:
@@ -264,34 +276,29 @@ def sample_adjusted(out: torch.Tensor, logits: torch.Tensor, temperature: Option
     `adjusted` float32 [M, V] receives l4 (it may be `logits`).  A vocabulary of at most 262,144."""
     if logits.dim() != 2:
         raise KernelError(f"logits must be [rows, vocabulary], got {tuple(logits.shape)}")
-    M, V = logits.shape
-    _want(logits, "logits", torch.float32)
-    _want(out, "out", torch.int32, (M,))
+    M, V = rows = logits.shape
+    i32, f32, each = torch.int32, torch.float32, (M,)
+    wanted = [(logits, "logits", f32, None), (out, "out", i32, each)]
     if temperature is not None:
         if seeds is None or counters is None:
             raise KernelError("temperature sampling needs seeds and counters")
-        _want(temperature, "temperature", torch.float32, (M,))
-        _want(seeds, "seeds", torch.int32, (M,))
-        _want(counters, "counters", torch.int32, (M,))
+        wanted += ((temperature, "temperature", f32, each), (seeds, "seeds", i32, each), (counters, "counters", i32, each))
     width = words = 0
     if history is not None or penalties is not None:
-        if any(t is None for t in (history, history_rows, prompt_lens, lengths, penalties)):
+        if history is None or history_rows is None or prompt_lens is None or lengths is None or penalties is None:
             raise KernelError("penalties need history, history_rows, prompt_lens, lengths and penalties")
         if history.dim() != 2 or history.shape[1] < 1:
             raise KernelError(f"history must be [rows, tokens], got {tuple(history.shape)}")
         width = history.shape[1]
-        _want(history, "history", torch.int32)
-        _want(history_rows, "history_rows", torch.int32, (M,))
-        _want(prompt_lens, "prompt_lens", torch.int32, (M,))
-        _want(lengths, "lengths", torch.int32, (M,))
-        _want(penalties, "penalties", torch.float32, (M, 3))
+        wanted += ((history, "history", i32, None), (history_rows, "history_rows", i32, each),
+                   (prompt_lens, "prompt_lens", i32, each), (lengths, "lengths", i32, each), (penalties, "penalties", f32, (M, 3)))
     if bias_starts is not None or bias_ids is not None or bias_values is not None:
-        if any(t is None for t in (bias_starts, bias_ids, bias_values)):
+        if bias_starts is None or bias_ids is None or bias_values is None:
             raise KernelError("biases need bias_starts, bias_ids and bias_values")
-        _want(bias_starts, "bias_starts", torch.int32, (M + 1,))
-        _want(bias_ids, "bias_ids", torch.int32, (bias_ids.numel(),))
-        _want(bias_values, "bias_values", torch.float32, (bias_ids.numel(),))
-        if bias_ids.numel() == 0:                           # nobody has a bias, and empty tensors have no address
+        n = bias_ids.numel()
+        wanted += ((bias_starts, "bias_starts", i32, (M + 1,)), (bias_ids, "bias_ids", i32, (n,)),
+                   (bias_values, "bias_values", f32, (n,)))
+        if n == 0:                                          # nobody has a bias, and empty tensors have no address
             bias_starts = bias_ids = bias_values = None
     if mask is not None or mask_rows is not None:
         if mask is None or mask_rows is None:
@@ -299,19 +306,16 @@ def sample_adjusted(out: torch.Tensor, logits: torch.Tensor, temperature: Option
         words = -(-V // 32)
         if mask.dim() != 2 or mask.shape[1] != words:
             raise KernelError(f"mask must be [masks, {words}], got {tuple(mask.shape)}")
-        _want(mask, "mask", torch.int32)
-        _want(mask_rows, "mask_rows", torch.int32, (M,))
+        wanted += ((mask, "mask", i32, None), (mask_rows, "mask_rows", i32, each))
     if adjusted is not None:
-        _want(adjusted, "adjusted", torch.float32, (M, V))
-    need = sample_scratch_size(M, V)
+        wanted.append((adjusted, "adjusted", f32, rows))
     if scratch is None:
-        scratch = torch.zeros(need, dtype=torch.int32, device=logits.device)
-    _want(scratch, "scratch", torch.int32)
-    if scratch.numel() < need:
-        raise KernelError(f"sample scratch has {scratch.numel()} entries, {need} are needed")
+        scratch = torch.zeros(sample_scratch_size(M, V), dtype=torch.int32, device=logits.device)
+    wanted.append((scratch, "scratch", i32, None))
+    _check(torch.cuda.current_device(), wanted)
     lib = library()
     check(lib, lib.sb_sample_adjusted(
-        _ptr(out), _ptr(logits), _ptr(temperature), _ptr(seeds), _ptr(counters), M, V, _ptr(scratch), _ptr(history), width,
+        _ptr(out), _ptr(logits), _ptr(temperature), _ptr(seeds), _ptr(counters), M, V, scratch.data_ptr(), scratch.numel(), _ptr(history), width,
         _ptr(history_rows), _ptr(prompt_lens), _ptr(lengths), _ptr(penalties), _ptr(bias_starts), _ptr(bias_ids),
         _ptr(bias_values), _ptr(mask), words, _ptr(mask_rows), _ptr(adjusted), _stream()), "sample_adjusted",
         kernels=1 if M else 0)
@@ -326,10 +330,7 @@ def copy_pages(k_pools: torch.Tensor, v_pools: torch.Tensor, src: Sequence[int],
     copies is two calls).  Kernels launched later on the stream, whatever they read early, find the copies done."""
     if k_pools.dim() != 5 or v_pools.dim() != 5 or k_pools.shape[:4] != v_pools.shape[:4]:
         raise KernelError(f"pools must be [runs, pages, heads, slots, dim], got {tuple(k_pools.shape)} and {tuple(v_pools.shape)}")
-    _want(k_pools, "k_pools")
-    _want(v_pools, "v_pools", k_pools.dtype)
-    if k_pools.device != v_pools.device:
-        raise KernelError("k_pools and v_pools must be on one device")
+    _check(torch.cuda.current_device(), ((k_pools, "k_pools", k_pools.dtype, None), (v_pools, "v_pools", k_pools.dtype, None)))
     n = len(src)
     if len(dst) != n:
         raise KernelError(f"{n} pages to copy and {len(dst)} places")
@@ -352,7 +353,7 @@ def copy_pages(k_pools: torch.Tensor, v_pools: torch.Tensor, src: Sequence[int],
 def attention_shared_scratch_size(members: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int,
                                   dtype: torch.dtype) -> Tuple[int, int]:
     """(float32, int32) entries of scratch that `attention_shared` needs for up to so many members, in at most as many
-    groups."""
+    groups; the int32 ones are zero before the first call."""
     floats, ints = ctypes.c_longlong(), ctypes.c_longlong()
     lib = library()
     check(lib, lib.sb_attention_shared_scratch(members, num_heads, num_kv_heads, head_dim, page_size, _code(dtype),
@@ -373,39 +374,37 @@ def attention_shared(out: torch.Tensor, q: torch.Tensor, k_pool: torch.Tensor, v
     token's own position are not seen).  A token that shares nothing is a group of its own with length 0.  Tokens in no
     group are left alone in `out`.  group_starts int32 [groups + 1] starts at 0; empty groups may stand anywhere.
 
-    Scratch: `part` float32 and `lists` int32 of attention_shared_scratch_size() entries, allocated here if None.
+    Scratch: `part` float32 and `lists` int32 of attention_shared_scratch_size() entries, allocated here if None; `lists` is
+    zero before its first use (the kernels leave it ready for the next call, of whatever shape).
     `status`: int32 word for the bounded waits of the tensor-core kernel, which is not used without it."""
     N = q.shape[0]
     if k_pool.dim() != 4:
         raise KernelError(f"k_pool must be [pages, heads, slots, dim], got {tuple(k_pool.shape)}")
     _, Hkv, BS, D = k_pool.shape
     Hq, M, R = num_heads, members.numel(), shared_lens.numel()
-    _code(q.dtype)
-    _want(q, "q", None, (N, Hq * D))
-    _want(out, "out", q.dtype, (N, Hq * D))
-    _want(k_pool, "k_pool", q.dtype)
-    _want(v_pool, "v_pool", q.dtype, k_pool.shape)
-    _want(block_table, "block_table", torch.int32)
+    dtype, i32, each, rows = _code(q.dtype), torch.int32, (N,), (N, Hq * D)
     if block_table.dim() != 2:
         raise KernelError(f"block_table must be [rows, pages], got {tuple(block_table.shape)}")
-    _want(token_rows, "token_rows", torch.int32, (N,))
-    _want(positions, "positions", torch.int32, (N,))
-    _want(members, "members", torch.int32, (M,))
-    _want(shared_lens, "shared_lens", torch.int32, (R,))
-    _want(group_starts, "group_starts", torch.int32, (R + 1,))
+    here = torch.cuda.current_device()
+    _check(here, ((q, "q", q.dtype, rows), (out, "out", q.dtype, rows), (k_pool, "k_pool", q.dtype, None),
+                  (v_pool, "v_pool", q.dtype, k_pool.shape), (block_table, "block_table", i32, None),
+                  (token_rows, "token_rows", i32, each), (positions, "positions", i32, each), (members, "members", i32, (M,)),
+                  (shared_lens, "shared_lens", i32, (R,)), (group_starts, "group_starts", i32, (R + 1,))))
     if M == 0 or R == 0:
         return
     if part is None or lists is None:
         floats, ints = attention_shared_scratch_size(M, Hq, Hkv, D, BS, q.dtype)
         part = torch.empty(floats, dtype=torch.float32, device=q.device) if part is None else part
-        lists = torch.empty(ints, dtype=torch.int32, device=q.device) if lists is None else lists
-    _want(part, "part", torch.float32)
-    _want(lists, "lists", torch.int32)
+        lists = torch.zeros(ints, dtype=torch.int32, device=q.device) if lists is None else lists
+    _check(here, ((part, "part", torch.float32, None), (lists, "lists", i32, None)))
+    if status is not None:
+        _check(here, ((status, "status", i32, None),))
     lib = library()
     check(lib, lib.sb_attention_shared(
         _ptr(out), _ptr(part), part.numel(), _ptr(lists), lists.numel(), _ptr(q), _ptr(k_pool), _ptr(v_pool),
-        _ptr(block_table), block_table.shape[1], _ptr(token_rows), _ptr(positions), _ptr(members), M, _ptr(group_starts), _ptr(shared_lens), R, N, Hq, Hkv, D, BS,
-        int(window), float(scale), _code(q.dtype), _stream()), "attention_shared", kernels=2)
+        k_pool.shape[0], _ptr(block_table), block_table.shape[1], _ptr(token_rows), _ptr(positions), _ptr(members), M, _ptr(group_starts), _ptr(shared_lens), R, N, Hq, Hkv, D, BS,
+        int(window), float(scale), dtype, _ptr(status), _stream()), "attention_shared",
+        kernels=lib.sb_attention_shared_kernels(M, R, Hq, Hkv, D, BS, k_pool.shape[0], status is not None))
 
 
 def gemm_simt(out: torch.Tensor, a: torch.Tensor, w: torch.Tensor, splits: int = 1, w_older: bool = False) -> None:

@@ -205,6 +205,8 @@ FAMILIES = {
     "no_own_keys": [(48, [0, 0, 5]), (37, [0, 3])],
     "more_rows_than_a_tile": [(100, list(range(1, 41)))],
     "long": [(1000, [1, 300, 64]), (500, [2, 2])],
+    "large_families": [(130, [3] * 20), (0, [9]), (1000, [1, 64] * 15), (16, [2] * 9)],
+    "a_hundred": [(400, [1, 30] * 50)],
 }
 
 
@@ -223,6 +225,27 @@ def test_attention_shared_windows(heads, window, dtype):
     """A window of 1 or 20 leaves most rows nothing of the prefix, one of 100 a part that differs by row."""
     case = Case([(96, [1, 5, 50, 200]), (160, [7] * 6 + [90]), (0, [40])], *heads, dtype, seed=window)
     check(case, case.run(window), case.want(window))
+
+
+def test_attention_shared_of_more_members_than_the_lists_in_shared_memory_hold():
+    case = Case([(32, [1, 3] * 300), (48, [2] * 3)], 4, 2, 32, torch.bfloat16, seed=8).poison()
+    check(case, case.run(), case.want())
+
+
+def test_attention_shared_large_families_with_windows():
+    case = Case([(300, [1, 5, 50, 200] * 5), (160, [7] * 17 + [90])], 32, 8, 128, torch.bfloat16, seed=2)
+    for window in (3, 150, 290):
+        check(case, case.run(window), case.want(window))
+
+
+@pytest.mark.parametrize("status", [True, False])
+def test_attention_shared_twice_is_the_same_bits(status):
+    """Nothing is added in the order in which blocks come; with and without the kernel for large families."""
+    case = Case([(1500, [1, 70, 9] * 8), (64, [40, 3])], 32, 8, 128, torch.bfloat16, seed=9)
+    first = case.run(status=status).clone()
+    for _ in range(20):
+        assert torch.equal(case.run(status=status), first)
+    check(case, first, case.want())
 
 
 @pytest.mark.parametrize("page", [1, 4, 32, 64, 128])
