@@ -261,19 +261,6 @@ void rows_parts(int M, int Hq, int Hkv, int num_sms, int* NP, int* NS) {
     *NS = *NS < 1 ? 1 : *NS > 8 ? 8 : *NS;
 }
 
-int sm_count() {
-    static sb::OncePerDevice asked;
-    static int count = 0;
-    bool& done = asked.flag();
-    if (!done) {
-        int dev = 0;
-        cudaGetDevice(&dev);
-        cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, dev);
-        done = true;
-    }
-    return count;
-}
-
 }  // namespace
 
 // Scratch of a call with up to M members in up to M families, in entries: float32, and int32.

@@ -65,6 +65,20 @@ struct OncePerDevice {
     }
 };
 
+// SMs of the current device.
+inline int sm_count() {
+    static OncePerDevice asked;
+    static int count[64] = {};
+    bool& done = asked.flag();
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!done) {
+        cudaDeviceGetAttribute(&count[dev & 63], cudaDevAttrMultiProcessorCount, dev);
+        done = true;
+    }
+    return count[dev & 63];
+}
+
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
                           Args&&... args) {

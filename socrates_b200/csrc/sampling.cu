@@ -26,12 +26,12 @@ __device__ __forceinline__ bool better(float v, int i, float best, int best_i) {
     return v > best || (v == best && i < best_i);
 }
 
-// The end of a block that looked through a slice of row m: its warps' best (in s_val, s_idx, behind a barrier) become the
-// slice's, and the row's last block to come merges the slices (see sample_kernel).
-__device__ __forceinline__ void merge_slices(int* __restrict__ out, int* __restrict__ scratch, int m, int C, float best,
-                                             int best_i, const float* s_val, const int* s_idx, int* s_last) {
+// The end of a block that looked through a part of row m: its warps' best (in s_val, s_idx, behind a barrier) become the
+// part's, and the last of the row's C blocks to come merges the parts (see sample_kernel).  `mine`: 2 C entries, `counter`: zero
+// before and after.
+__device__ __forceinline__ void merge_slices(int* __restrict__ out, int* __restrict__ mine, int* __restrict__ counter, int m, int C,
+                                             float best, int best_i, const float* s_val, const int* s_idx, int* s_last) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int* mine = scratch + (size_t)m * (2 * C + 1);
     if (warp == 0) {
         const int nw = (blockDim.x + 31) >> 5;
         best = lane < nw ? s_val[lane] : -INFINITY;
@@ -46,7 +46,7 @@ __device__ __forceinline__ void merge_slices(int* __restrict__ out, int* __restr
             mine[2 * blockIdx.y] = __float_as_int(best);
             mine[2 * blockIdx.y + 1] = best_i;
             __threadfence();
-            *s_last = atomicAdd(&mine[2 * C], 1) == C - 1;
+            *s_last = atomicAdd(counter, 1) == C - 1;
         }
     }
     __syncthreads();
@@ -69,7 +69,7 @@ __device__ __forceinline__ void merge_slices(int* __restrict__ out, int* __restr
         if (lane == 0) {
             // A row of NaNs or -inf leaves best_i untouched; report index 0 rather than garbage.
             out[m] = best_i == 0x7fffffff ? 0 : best_i;
-            mine[2 * C] = 0;
+            *counter = 0;
         }
     }
 }
@@ -143,7 +143,8 @@ __global__ void sample_kernel(int* __restrict__ out, const float* __restrict__ l
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (lane == 0) { s_val[warp] = best; s_idx[warp] = best_i; }
     __syncthreads();
-    merge_slices(out, scratch, m, C, best, best_i, s_val, s_idx, &s_last);
+    int* mine = scratch + (size_t)m * (2 * C + 1);
+    merge_slices(out, mine, mine + 2 * C, m, C, best, best_i, s_val, s_idx, &s_last);
 }
 
 // What a row's logits go through before they are compared: with c the number of times a token stands in the row's output
@@ -151,8 +152,8 @@ __global__ void sample_kernel(int* __restrict__ out, const float* __restrict__ l
 //   l1 = met ? (l > 0 ? l / repetition : l * repetition) : l
 //   l2 = l1 - frequency * c - presence * (c > 0),   l3 = l2 + bias,   l4 = allowed ? l3 : -inf.
 struct Adjust {
-    const int *history, *history_rows, *prompt_lens, *lengths;      // tokens [rows, width]; null: no penalties
-    const float* penalties;                                         // [M, 3]: repetition, presence, frequency
+    const int *history, *history_rows, *prompt_lens, *lengths;      // tokens [rows, width]
+    const float* penalties;                                         // [M, 3]: repetition, presence, frequency; null: none
     const int *bias_starts, *bias_ids;                              // null: no biases
     const float* bias_values;
     const uint32_t* mask;                                           // [rows, words]; null: no masks
@@ -161,71 +162,56 @@ struct Adjust {
     int history_width, mask_words;
 };
 
-constexpr int SLICE = 8192;          // logits of a block, whose counts and biases are held in shared memory
+constexpr int SLICE = 8192;          // logits of a block at most, held in shared memory with their tokens' counts
 
-// sample_kernel with adjusted logits.  A block counts the row's tokens that fall into its slice (integer atomics in shared
-// memory: the order does not matter), so no table as wide as the vocabulary is kept from step to step.  What bounds it: the
-// logits' bytes and, for rows that draw, two logarithms a logit.  A thread holds its 16 logits in registers, loaded (16 bytes
-// each where rows allow it) before the counts are made; logits of tokens that a mask forbids are not read.
+// sample_kernel with adjusted logits.  What bounds it: the logits' bytes, and instructions.  A block brings a slice of a row to
+// shared memory and marks in a table beside it which of the slice's tokens the row's tokens and biases name, and how often
+// (integer atomics in shared memory: the order does not matter, and no table as wide as the vocabulary is kept from step to step).
+// Then whoever named a token takes its mark out of the table, which one thread gets, and adjusts its logit: few logits are met,
+// and the scan that follows is a plain one.  Logits of tokens that a mask forbids are not read, four at a time.  Blocks are
+// small (three an SM), so that the phases of one, which wait for one another, run beside those of others.
 //
 // A row that draws needs the noise of few logits: with N = 2^23 - (hash >> 9) in [1, 2^23] the noise -log(-log(u)) is at most
-// -log(1 - u) = log(2^23 / (N - 1/2)).  A block first takes the largest of the scores of its threads' largest logits; a logit l
-// can exceed that, F, only where N - 1/2 <= 2^23 e^(l / T - F), and the others are not looked at.
-// 64 rows of 151,936 logits, half of them drawn, tokens of up to 4,096 and 40 biases a row: 60 us a logit at a time, 42 so.
-__global__ void __launch_bounds__(512, 2)
+// -log(1 - u) = log(2^23 / (N - 1/2)).  A block first takes the largest of the scores of its threads' largest logits, F; a logit that is at
+// most l can exceed it only where N - 1/2 <= 2^23 e^(l / T - F), a bound on the hash that a thread takes once, with its
+// largest logit.  The others are not looked at.
+// 64 rows of 151,936 logits, half of them drawn, tokens of up to 4,096 and 40 biases a row: 60 us a logit at a time with tables for
+// counts and biases, 42 with 16 logits a thread in registers, 31 so (22 if none is drawn, 14 if nothing is adjusted either).
+__global__ void __launch_bounds__(512, 3)
 sample_adjusted_kernel(int* __restrict__ out, const float* __restrict__ logits, const float* __restrict__ temperature,
                        const uint32_t* __restrict__ seeds, const uint32_t* __restrict__ counters, int V, int per,
-                       int* __restrict__ scratch, const Adjust a) {
+                       int* __restrict__ scratch_end, const Adjust a) {
     sb::pdl_launch_dependents();
     sb::pdl_wait();
+    constexpr int THREADS = 512, J = SLICE / (4 * THREADS), AT = 2;
+    constexpr int PROMPT = (int)0x80000000u, BIASED = 0x40000000, TWICE = 0x20000000, MADE = TWICE - 1;
     extern __shared__ __align__(16) uint8_t smem[];
-    int* count = reinterpret_cast<int*>(smem);              // [per]: bit 31 "stands in the prompt", below it c
-    float* bias = reinterpret_cast<float*>(smem) + (a.history != nullptr ? per : 0);      // [per]
+    float* lg = reinterpret_cast<float*>(smem);             // [per] the slice's logits
+    int* marks = reinterpret_cast<int*>(lg + per);          // [per]: PROMPT, BIASED, TWICE (so), times in the output
     __shared__ float s_val[32];
     __shared__ int s_idx[32];
     __shared__ int s_last;
-    constexpr int THREADS = 512, J = SLICE / (4 * THREADS);  // four times four logits a thread
-    const int m = blockIdx.x, C = gridDim.y, tid = threadIdx.x;
+    const int m = blockIdx.x, slices = gridDim.y, tid = threadIdx.x;
     const int lane = tid & 31, warp = tid >> 5;
     const float* row = logits + (size_t)m * V;
-    const int begin = min(V, (int)blockIdx.y * per), end = min(V, begin + per);
-    // logit (j, e) of a thread is `at + 2048 j + step e`: neighbours where 16-byte loads are possible
+    const int begin = min(V, (int)blockIdx.y * per), n = min(V, begin + per) - begin;
     const bool wide = V % 4 == 0 && ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(a.adjusted)) & 15) == 0;
-    const int at = begin + (wide ? 4 * tid : tid), step = wide ? 1 : THREADS;
 
-    const int mask_row = a.mask != nullptr ? a.mask_rows[m] : -1;
-    uint32_t may = 0xffffu;                                 // bit 4 j + e: the token is allowed
-    if (mask_row >= 0) {
-        const uint32_t* allowed = a.mask + (size_t)mask_row * a.mask_words;
-        may = 0;
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-            const int i = at + 4 * THREADS * j;
-            if (wide) {
-                if (i < end) may |= (allowed[i >> 5] >> (i & 31) & 15u) << (4 * j);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (i + step * e < end) may |= (allowed[(i + step * e) >> 5] >> ((i + step * e) & 31) & 1u) << (4 * j + e);
-            }
-        }
+    const bool penal = a.penalties != nullptr, biased = a.bias_starts != nullptr;
+    const int* told = nullptr;
+    int len = 0, prompt = 0, bias0 = 0, bias1 = 0;
+    float rep = 1.f, presence = 0.f, frequency = 0.f;
+    if (penal) {
+        told = a.history + (size_t)a.history_rows[m] * a.history_width;
+        len = min(a.lengths[m], a.history_width);
+        prompt = a.prompt_lens[m];
+        rep = a.penalties[3 * m];
+        presence = a.penalties[3 * m + 1];
+        frequency = a.penalties[3 * m + 2];
     }
-    // a place behind the slice holds NaN, which is never the best, one that is not allowed -inf
-    float v[4 * J];
-    const float none = __int_as_float(0x7fffffff);
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-        const int i = at + 4 * THREADS * j;
-        float4 x = make_float4(none, none, none, none);
-        if (wide) {
-            if (i < end) x = may >> (4 * j) & 15u ? *reinterpret_cast<const float4*>(row + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-        } else {
-            if (i < end) x.x = row[i];
-            if (i + step < end) x.y = row[i + step];
-            if (i + 2 * step < end) x.z = row[i + 2 * step];
-            if (i + 3 * step < end) x.w = row[i + 3 * step];
-        }
-        v[4 * j] = x.x; v[4 * j + 1] = x.y; v[4 * j + 2] = x.z; v[4 * j + 3] = x.w;
+    if (biased) {
+        bias0 = a.bias_starts[m];
+        bias1 = a.bias_starts[m + 1];
     }
     const float T = temperature ? temperature[m] : 0.f;
     uint32_t key = 0;
@@ -233,124 +219,174 @@ sample_adjusted_kernel(int* __restrict__ out, const float* __restrict__ logits, 
         key = mix32(seeds[m] ^ 0x9E3779B9u);
         key = mix32(key ^ mix32(counters[m] + 0x85EBCA6Bu));
     }
-    const float inv_t = T > 0.f ? 1.0f / T : 1.0f;
 
-    // ---- counts and biases of the slice's tokens
-    const bool penal = a.history != nullptr, biased = a.bias_starts != nullptr;
-    if (penal || biased) {
-        const int4 zero = make_int4(0, 0, 0, 0);
-        for (int i = 4 * tid; i < per * (penal + biased); i += 4 * THREADS) *reinterpret_cast<int4*>(count + i) = zero;
-        __syncthreads();
-    }
-    float rep = 1.f, presence = 0.f, frequency = 0.f;
-    const int n = end - begin;
-    if (penal) {
-        rep = a.penalties[3 * m];
-        presence = a.penalties[3 * m + 1];
-        frequency = a.penalties[3 * m + 2];
-        const int* told = a.history + (size_t)a.history_rows[m] * a.history_width;
-        const int len = min(a.lengths[m], a.history_width), prompt = a.prompt_lens[m];
-        constexpr int AT = 8;                               // loads in flight
-        for (int i0 = tid; i0 < len; i0 += AT * THREADS) {
-            int t[AT];
-#pragma unroll
-            for (int u = 0; u < AT; ++u) t[u] = i0 + u * THREADS < len ? told[i0 + u * THREADS] - begin : -1;
-#pragma unroll
-            for (int u = 0; u < AT; ++u)
-                if (t[u] >= 0 && t[u] < n) {
-                    if (i0 + u * THREADS < prompt) atomicOr(&count[t[u]], (int)0x80000000u);
-                    else atomicAdd(&count[t[u]], 1);
-                }
-        }
-    }
-    if (biased && warp == THREADS / 32 - 1) {
-        // in the order of the list, so that a token named twice gets both in that order
-        const int e1 = a.bias_starts[m + 1];
-        for (int e0 = a.bias_starts[m]; e0 < e1; e0 += 32) {
-            const int t = e0 + lane < e1 ? a.bias_ids[e0 + lane] - begin : -1;
-            const float x = e0 + lane < e1 ? a.bias_values[e0 + lane] : 0.f;
-            const bool mine = t >= 0 && t < n;
-            const uint32_t same = __match_any_sync(0xffffffffu, mine ? t : -1 - lane);
-            const int rank = __popc(same & ((1u << lane) - 1u));
-            const int rounds = __reduce_max_sync(0xffffffffu, rank);
-            for (int r = 0; r <= rounds; ++r) {
-                if (mine && rank == r) bias[t] += x;
-                __syncwarp();
-            }
-        }
-    }
-    if (penal || biased) __syncthreads();
-
-    // ---- the adjusted logits
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-        const int i = at + 4 * THREADS * j;
-        if (penal && i < end) {
-            int c[4] = {0, 0, 0, 0};
-            if (wide) {
-                const int4 x = *reinterpret_cast<const int4*>(count + i - begin);
-                c[0] = x.x; c[1] = x.y; c[2] = x.z; c[3] = x.w;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (i + step * e < end) c[e] = count[i + step * e - begin];
-            }
-            if (c[0] | c[1] | c[2] | c[3]) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (c[e] != 0) {
-                        float x = v[4 * j + e];
-                        x = x > 0.f ? x / rep : x * rep;
-                        const int made = c[e] & 0x7fffffff;
-                        v[4 * j + e] = made > 0 ? x - frequency * (float)made - presence : x;
-                    }
-            }
-        }
-        if (biased && i < end) {
-            if (wide) {
-                const float4 x = *reinterpret_cast<const float4*>(bias + i - begin);
-                v[4 * j] += x.x; v[4 * j + 1] += x.y; v[4 * j + 2] += x.z; v[4 * j + 3] += x.w;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (i + step * e < end) v[4 * j + e] += bias[i + step * e - begin];
-            }
-        }
-    }
+    // four logits a thread and round: 4 (tid + 512 j) .. + 3 of the slice.  `begin` is a multiple of 4: the four lie in one word of
+    // the mask.
+    const int mask_row = a.mask != nullptr ? a.mask_rows[m] : -1;
+    uint32_t may = 0xffffu;                                 // bit 4 j + e: the token is allowed
     if (mask_row >= 0) {
-#pragma unroll
-        for (int k = 0; k < 4 * J; ++k)
-            if (!(may >> k & 1u) && at + 4 * THREADS * (k / 4) + step * (k % 4) < end) v[k] = -INFINITY;
-    }
-    if (a.adjusted != nullptr) {
-        float* to = a.adjusted + (size_t)m * V;
+        const uint32_t* allowed = a.mask + (size_t)mask_row * a.mask_words;
+        may = 0;
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            const int i = at + 4 * THREADS * j;
+            const int i = 4 * (tid + THREADS * j);
+            if (i < n) may |= (allowed[(begin + i) >> 5] >> ((begin + i) & 31) & 15u) << (4 * j);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        const int i = 4 * (tid + THREADS * j);
+        const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(lg + i));
+        if (i < n && (may >> (4 * j) & 15u)) {
             if (wide) {
-                if (i < end) *reinterpret_cast<float4*>(to + i) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(row + begin + i) : "memory");
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (i + step * e < end) to[i + step * e] = v[4 * j + e];
+                    if (i + e < n)
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + 4 * e), "l"(row + begin + i + e) : "memory");
             }
         }
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
 
-    // ---- the best of them.  A thread's places come in the order of their indices, so the first of equal ones stays.
+    if (penal || biased) {
+        const bool wide_told = (reinterpret_cast<uintptr_t>(told) & 15) == 0;
+        auto tokens = [&](int i) {                          // four from i on, less `begin`; behind the row's last one: none
+            int4 x = make_int4(-1, -1, -1, -1);
+            if (wide_told && i + 3 < len) {
+                x = *reinterpret_cast<const int4*>(told + i);
+            } else {
+                if (i < len) x.x = told[i];
+                if (i + 1 < len) x.y = told[i + 1];
+                if (i + 2 < len) x.z = told[i + 2];
+                if (i + 3 < len) x.w = told[i + 3];
+            }
+            x.x -= begin; x.y -= begin; x.z -= begin; x.w -= begin;
+            return x;
+        };
+        int4 t[AT];                                         // the first 4,096 tokens
+#pragma unroll
+        for (int u = 0; u < AT; ++u) t[u] = tokens(4 * (tid + u * THREADS));
+        // the first 512 biases, one a thread
+        int named = -1;
+        float bias = 0.f;
+        if (bias0 + tid < bias1) {
+            named = a.bias_ids[bias0 + tid] - begin;
+            bias = a.bias_values[bias0 + tid];
+        }
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+            if (4 * (tid + THREADS * j) < per) reinterpret_cast<int4*>(marks)[tid + THREADS * j] = make_int4(0, 0, 0, 0);
+        __syncthreads();
+        // f(token - begin, place in the list) for the row's tokens that lie in the slice, f(token - begin, bias) for its biases.
+        // (A token outside the vocabulary lies in no slice: what it is less `begin` is negative or, wrapped round, far too large.)
+        auto each = [&](auto f) {
+            auto one = [&](int x, int i) {
+                if ((unsigned)x < (unsigned)n) f(x, i);
+            };
+            auto four = [&](const int4& x, int i) { one(x.x, i); one(x.y, i + 1); one(x.z, i + 2); one(x.w, i + 3); };
+#pragma unroll
+            for (int u = 0; u < AT; ++u) four(t[u], 4 * (tid + u * THREADS));
+            for (int i0 = AT * THREADS; 4 * i0 < len; i0 += AT * THREADS) {
+                int4 x[AT];
+#pragma unroll
+                for (int u = 0; u < AT; ++u) x[u] = tokens(4 * (i0 + tid + u * THREADS));
+#pragma unroll
+                for (int u = 0; u < AT; ++u) four(x[u], 4 * (i0 + tid + u * THREADS));
+            }
+        };
+        auto each_bias = [&](auto f) {
+            if ((unsigned)named < (unsigned)n) f(named, bias);
+            for (int e = bias0 + THREADS + tid; e < bias1; e += THREADS) {
+                const int x = a.bias_ids[e] - begin;
+                if ((unsigned)x < (unsigned)n) f(x, a.bias_values[e]);
+            }
+        };
+        each([&](int x, int i) {
+            if (i < prompt) atomicOr(&marks[x], PROMPT);
+            else atomicAdd(&marks[x], 1);
+        });
+        each_bias([&](int x, float) {
+            if (atomicOr(&marks[x], BIASED) & BIASED) atomicOr(&marks[x], TWICE);
+        });
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();
+        const float inv_rep = 1.0f / rep;
+        auto adjust = [&](int x, bool knows, float value) {
+            const int c = atomicExch(&marks[x], 0);          // whoever else names this token gets 0
+            if (c == 0) return;
+            float l = lg[x];
+            const int made = c & MADE;
+            if (c & (PROMPT | MADE)) l *= l > 0.f ? inv_rep : rep;
+            if (made > 0) l = l - frequency * (float)made - presence;
+            if (c & BIASED) {
+                if (knows && !(c & TWICE)) l += value;
+                else                                        // in the order of the list: a token named twice gets both so
+                    for (int e = bias0; e < bias1; ++e)
+                        if (a.bias_ids[e] == begin + x) l += a.bias_values[e];
+            }
+            lg[x] = l;
+        };
+        each_bias([&](int x, float value) { adjust(x, true, value); });
+        each([&](int x, int) { adjust(x, false, 0.f); });
+    } else {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
+    __syncthreads();
+
+    // ---- the scan.  A place behind the slice holds NaN, which is never the best, one that is not allowed -inf.  A thread's places
+    // come in the order of their indices: the first of equal ones stays.
+    const float none = __int_as_float(0x7fffffff);
+    auto four = [&](int j) {
+        const int i = 4 * (tid + THREADS * j);
+        float4 x = make_float4(none, none, none, none);
+        if (i < n) x = *reinterpret_cast<const float4*>(lg + i);
+        if (mask_row >= 0) {
+            if (!(may >> (4 * j) & 1u)) x.x = -INFINITY;
+            if (!(may >> (4 * j) & 2u)) x.y = -INFINITY;
+            if (!(may >> (4 * j) & 4u)) x.z = -INFINITY;
+            if (!(may >> (4 * j) & 8u)) x.w = -INFINITY;
+        }
+        if (i + 3 >= n) {
+            if (i >= n) x.x = none;
+            if (i + 1 >= n) x.y = none;
+            if (i + 2 >= n) x.z = none;
+            x.w = none;
+        }
+        return x;
+    };
     float best = -INFINITY;
     int best_k = -1;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        const float4 x = four(j);
+        if (x.x > best) { best = x.x; best_k = 4 * j; }
+        if (x.y > best) { best = x.y; best_k = 4 * j + 1; }
+        if (x.z > best) { best = x.z; best_k = 4 * j + 2; }
+        if (x.w > best) { best = x.w; best_k = 4 * j + 3; }
+        if (a.adjusted != nullptr) {
+            const int i = 4 * (tid + THREADS * j);
+            float* to = a.adjusted + (size_t)m * V + begin + i;
+            if (wide) {
+                if (i < n) *reinterpret_cast<float4*>(to) = x;
+            } else {
+                if (i < n) to[0] = x.x;
+                if (i + 1 < n) to[1] = x.y;
+                if (i + 2 < n) to[2] = x.z;
+                if (i + 3 < n) to[3] = x.w;
+            }
+        }
+    }
+    const int first = begin + 4 * tid;
+    auto place = [&](int k) { return first + 4 * THREADS * (k >> 2) + (k & 3); };
     if (T > 0.f) {
+        const float inv_t = 1.0f / T;
         auto score = [&](float x, int k) {                  // as sample_kernel's, operation by operation
-            const float u = uniform_for(key, (uint32_t)(at + 4 * THREADS * (k / 4) + step * (k % 4)));
+            const float u = uniform_for(key, (uint32_t)place(k));
             return x * inv_t - logf(-logf(u));
         };
-        float top = -INFINITY;
-        int top_k = -1;
-#pragma unroll
-        for (int k = 0; k < 4 * J; ++k)
-            if (v[k] > top) { top = v[k]; top_k = k; }
-        float least = top_k >= 0 ? score(top, top_k) : -INFINITY;
+        float least = best_k >= 0 ? score(best, best_k) : -INFINITY;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) least = fmaxf(least, __shfl_xor_sync(0xffffffffu, least, o));
         if (lane == 0) s_val[warp] = least;
@@ -358,38 +394,30 @@ sample_adjusted_kernel(int* __restrict__ out, const float* __restrict__ logits, 
         least = s_val[lane & (THREADS / 32 - 1)];
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) least = fmaxf(least, __shfl_xor_sync(0xffffffffu, least, o));
-        // l / T in units of log2, less F, and 23: the exponent of the largest N.  2e-3 and 2e-6 of a score are far more than the
-        // roundings on both sides.
+        // The bound on N and from it the one on the hash.  The exponent is enlarged by 2e-3 and 4e-6 of its terms, far more than the
+        // roundings on both sides; whatever is not finite looks at everything.
         constexpr float LOG2E = 1.4426950408889634f;
-        const float slope = inv_t * LOG2E, offset = 23.0f + 2e-3f + 2e-6f * fabsf(least) - least * LOG2E;
+        const float l = best * inv_t, exponent = (l - least) * LOG2E + 2e-3f + 4e-6f * (fabsf(l) + fabsf(least));
+        const float bound = exponent < 0.f ? exp2f(23.0f + exponent) + 1.0f : 8388608.0f;
+        const uint32_t hash = (8388608u - (uint32_t)fminf(bound, 8388608.0f)) << 9;
         uint32_t look = 0;
+        if (best_k >= 0) {                                  // else nothing of this thread's can win
 #pragma unroll
-        for (int k = 0; k < 4 * J; ++k) {
-            const uint32_t i = (uint32_t)(at + 4 * THREADS * (k / 4) + step * (k % 4));
-            const float N = (float)(8388608u - (mix32((i + 0x165667B1u) ^ key) >> 9));
-            const float exponent = fmaf(v[k], slope, offset);
-            float most;
-            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(most) : "f"(fmaf(fabsf(exponent), 2e-6f, exponent)));
-            if (!(N - 0.5f > most)) look |= 1u << k;        // NaN and infinities are looked at
+            for (int k = 0; k < 4 * J; ++k)
+                if (mix32(((uint32_t)place(k) + 0x165667B1u) ^ key) >= hash) look |= 1u << k;
         }
-        while (__any_sync(0xffffffffu, look != 0)) {         // in the order of the places
+        best = -INFINITY;
+        best_k = -1;
+        while (look != 0) {                                 // in the order of the places
             const int k = __ffs(look) - 1;
-            if (k >= 0) {
-                float x = v[0];
-#pragma unroll
-                for (int y = 1; y < 4 * J; ++y) x = k == y ? v[y] : x;
-                x = score(x, k);
-                if (x > best) { best = x; best_k = k; }
-                look &= look - 1;
-            }
+            look &= look - 1;
+            const float4 x = four(k >> 2);
+            const float y = score((k & 3) == 0 ? x.x : (k & 3) == 1 ? x.y : (k & 3) == 2 ? x.z : x.w, k);
+            if (y > best) { best = y; best_k = k; }
         }
         __syncthreads();                                    // s_val is written again below
-    } else {
-#pragma unroll
-        for (int k = 0; k < 4 * J; ++k)
-            if (v[k] > best) { best = v[k]; best_k = k; }
     }
-    int best_i = best_k < 0 ? 0x7fffffff : at + 4 * THREADS * (best_k >> 2) + step * (best_k & 3);
+    int best_i = best_k < 0 ? 0x7fffffff : place(best_k);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         const float ov = __shfl_xor_sync(0xffffffffu, best, o);
@@ -398,7 +426,9 @@ sample_adjusted_kernel(int* __restrict__ out, const float* __restrict__ logits, 
     }
     if (lane == 0) { s_val[warp] = best; s_idx[warp] = best_i; }
     __syncthreads();
-    merge_slices(out, scratch, m, C, best, best_i, s_val, s_idx, &s_last);
+    // rows from the end of the scratch: what sample_kernel left at its beginning is not met
+    int* mine = scratch_end - (size_t)(m + 1) * (2 * slices + 1);
+    merge_slices(out, mine, mine + 2 * slices, m, slices, best, best_i, s_val, s_idx, &s_last);
 }
 
 }  // namespace
@@ -407,6 +437,12 @@ sample_adjusted_kernel(int* __restrict__ out, const float* __restrict__ logits, 
 extern "C" int sb_sample_slices(int V) {
     int c = (V + 8191) / 8192;
     return c < 1 ? 1 : (c > 32 ? 32 : c);
+}
+
+// The same for sb_sample_adjusted.
+extern "C" int sb_sample_adjusted_slices(int V) {
+    int c = (V + SLICE - 1) / SLICE;
+    return c < 1 ? 1 : c;
 }
 
 // scratch: int32, at least M * (2 * sb_sample_slices(V) + 1) entries, zero before the first use.
@@ -436,20 +472,21 @@ extern "C" int sb_sample_adjusted(int* out, const float* logits, const float* te
     SB_REQUIRE(M >= 0 && V > 0, "sample_adjusted: bad sizes M=%d V=%d", M, V);
     SB_REQUIRE(temperature == nullptr || (seeds != nullptr && counters != nullptr),
                "sample_adjusted: temperature sampling needs seeds and counters");
-    SB_REQUIRE(scratch != nullptr && scratch_ints >= (long long)M * (2 * sb_sample_slices(V) + 1),
-               "sample_adjusted: scratch has %lld entries, %lld are needed", scratch_ints, (long long)M * (2 * sb_sample_slices(V) + 1));
     SB_REQUIRE(V <= 32 * SLICE, "sample_adjusted: a vocabulary of %d (at most %d)", V, 32 * SLICE);
-    SB_REQUIRE(history == nullptr || (history_width > 0 && history_rows != nullptr && prompt_lens != nullptr &&
-                                      lengths != nullptr && penalties != nullptr),
+    SB_REQUIRE(M <= 65535 * 32, "sample_adjusted: too many rows");
+    const int slices = sb_sample_adjusted_slices(V);
+    SB_REQUIRE(scratch != nullptr && scratch_ints >= (long long)M * (2 * sb_sample_slices(V) + 1 + 2 * slices + 1),
+               "sample_adjusted: scratch has %lld entries, %lld are needed", scratch_ints,
+               (long long)M * (2 * sb_sample_slices(V) + 1 + 2 * slices + 1));
+    SB_REQUIRE(penalties == nullptr || (history != nullptr && history_width > 0 && history_rows != nullptr && prompt_lens != nullptr &&
+                                      lengths != nullptr),
                "sample_adjusted: penalties need the rows' tokens, their lengths and the three numbers of each row");
     SB_REQUIRE(bias_starts == nullptr || (bias_ids != nullptr && bias_values != nullptr), "sample_adjusted: biases need ids and values");
     SB_REQUIRE(mask == nullptr || (mask_rows != nullptr && mask_words == (V + 31) / 32), "sample_adjusted: masks of %d words for %d tokens", mask_words, V);
     if (M == 0) return 0;
-    const int C = sb_sample_slices(V);
-    const int per = ((V + C - 1) / C + 3) & ~3;
+    const int per = ((V + slices - 1) / slices + 3) & ~3;
     const Adjust a{history, history_rows, prompt_lens, lengths, penalties, bias_starts, bias_ids, bias_values, (const uint32_t*)mask,
                    mask_rows, adjusted, history_width, mask_words};
-    const int smem = per * 4 * ((history != nullptr) + (bias_starts != nullptr));
     static sb::OncePerDevice once_per_device;
     bool& configured = once_per_device.flag();
     if (!configured) {
@@ -457,7 +494,8 @@ extern "C" int sb_sample_adjusted(int* out, const float* logits, const float* te
         if (e != cudaSuccess) { sb_set_error("sample_adjusted: %s", cudaGetErrorString(e)); return (int)e; }
         configured = true;
     }
-    sb::launch(sample_adjusted_kernel, dim3(M, C), dim3(512), smem, stream, out, logits, temperature, seeds, counters, V, per,
-               scratch, a);
+    const int smem = per * 4 * (1 + (penalties != nullptr || bias_starts != nullptr));
+    sb::launch(sample_adjusted_kernel, dim3(M, slices), dim3(512), smem, stream, out, logits, temperature, seeds, counters, V, per,
+               scratch + scratch_ints, a);
     SB_LAUNCH_CHECK();
 }

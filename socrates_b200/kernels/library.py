@@ -37,6 +37,7 @@ _SIGNATURES = {
     "sb_silu_mul": [P, P, I, I, I, I, I, P],
     "sb_sample": [P, P, P, P, P, I, I, P, P],
     "sb_sample_slices": [I],
+    "sb_sample_adjusted_slices": [I],
     "sb_sample_adjusted": [P, P, P, P, P, I, I, P, LL, P, I, P, P, P, P, P, P, P, P, I, P, P, P],
     "sb_copy_pages": [P, P, P, P, I, I, I, LL, LL, P],
     "sb_copy_pages_kernels": [I],

@@ -218,8 +218,10 @@ def silu_mul(out: torch.Tensor, gate_up: torch.Tensor, interleaved: bool = False
 
 
 def sample_scratch_size(M: int, V: int) -> int:
-    """int32 entries of scratch that `sample` needs for M rows of V logits."""
-    return M * (2 * library().sb_sample_slices(int(V)) + 1)
+    """int32 entries of scratch that `sample` and `sample_adjusted` need for M rows of V logits (a place each: calls of both
+    may share it)."""
+    lib = library()
+    return M * (2 * lib.sb_sample_slices(int(V)) + 1 + 2 * lib.sb_sample_adjusted_slices(int(V)) + 1)
 
 
 def sample(out: torch.Tensor, logits: torch.Tensor, temperature: Optional[torch.Tensor] = None,
@@ -268,7 +270,7 @@ def sample_adjusted(out: torch.Tensor, logits: torch.Tensor, temperature: Option
     out[m] is what `sample` gives for l4 (0 for a row in which nothing is left).  Each of the three parts may be absent:
     * penalties float32 [M, 3] (repetition > 0, presence, frequency) over `history` int32 [rows, width]: row
       history_rows[m] holds lengths[m] tokens, of which the first prompt_lens[m] are the prompt (int32 [M] each; tokens
-      outside the vocabulary are passed over);
+      outside the vocabulary are passed over).  Without penalties the history is not looked at;
     * biases of row m: bias_values[i] (float32) on token bias_ids[i] (int32), i from bias_starts[m] to bias_starts[m + 1] - 1
       (int32 [M + 1]); a token named twice gets both;
     * `mask` int32 [masks, ceil(V / 32)]: bit t % 32 of word t // 32 allows token t; mask_rows[m] (int32 [M]) is the row's
@@ -284,9 +286,9 @@ def sample_adjusted(out: torch.Tensor, logits: torch.Tensor, temperature: Option
             raise KernelError("temperature sampling needs seeds and counters")
         wanted += ((temperature, "temperature", f32, each), (seeds, "seeds", i32, each), (counters, "counters", i32, each))
     width = words = 0
-    if history is not None or penalties is not None:
-        if history is None or history_rows is None or prompt_lens is None or lengths is None or penalties is None:
-            raise KernelError("penalties need history, history_rows, prompt_lens, lengths and penalties")
+    if penalties is not None:
+        if history is None or history_rows is None or prompt_lens is None or lengths is None:
+            raise KernelError("penalties need history, history_rows, prompt_lens and lengths")
         if history.dim() != 2 or history.shape[1] < 1:
             raise KernelError(f"history must be [rows, tokens], got {tuple(history.shape)}")
         width = history.shape[1]
