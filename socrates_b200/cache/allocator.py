@@ -5,6 +5,9 @@ usable pages are numbered 1..num_pages, page 0 stands for "no page" and never le
 the page given back last is handed out first, a request for more pages than are free
 changes nothing, and a `free` that names a bad page changes nothing either.
 
+Beyond that contract a page may have several holders (`share`): `free` takes one of them away, and the page is in again
+when the last one is gone.
+
 The form is this engine's own: a fixed stack of page numbers with a fill mark, and
 one state byte per page.  The byte answers "is this page out?" in O(1), which is
 what `free`, `holds` and `check` are built on; a cache group with hundreds of
@@ -14,7 +17,7 @@ thousands of pages allocates nothing after construction.
 from __future__ import annotations
 
 from array import array
-from typing import Iterable, List
+from typing import Dict, Iterable, List
 
 _IN, _OUT, _LEAVING = 0, 1, 2        # page state: in the stack, held by a row, named by the free() in progress
 
@@ -41,6 +44,7 @@ class PageAllocator:
         self._fill = num_pages
         self._state = bytearray(num_pages + 1)
         self._state[self.NULL] = _LEAVING                 # never in, never out: no transition accepts it
+        self._more: Dict[int, int] = {}                   # page -> holders beside the first, where there are any
 
     @property
     def n_free(self) -> int:
@@ -53,6 +57,19 @@ class PageAllocator:
     def holds(self, page: int) -> bool:
         """Whether `page` is out (held by somebody) right now."""
         return 0 < page <= self.num_pages and self._state[page] == _OUT
+
+    def holders(self, page: int) -> int:
+        """How many hold `page` (0: it is in, or no page of this pool)."""
+        return 1 + self._more.get(page, 0) if self.holds(page) else 0
+
+    def share(self, pages: Iterable[int]) -> None:
+        """One more holder for each of these pages, which are out; `free` takes it away again."""
+        pages = [int(p) for p in pages]
+        for p in pages:
+            if not self.holds(p):
+                raise ValueError(f"page {p} is not out: there is nobody to share it with")
+        for p in pages:
+            self._more[p] = self._more.get(p, 0) + 1
 
     def alloc(self, n: int) -> List[int]:
         if n < 0:
@@ -79,6 +96,14 @@ class PageAllocator:
             self._state[p] = _LEAVING
         # pushed back to front, so the pages come out again in the order they were named
         for p in reversed(pages):
+            more = self._more.get(p, 0)
+            if more:                                        # somebody else holds it still
+                if more == 1:
+                    del self._more[p]
+                else:
+                    self._more[p] = more - 1
+                self._state[p] = _OUT
+                continue
             self._stack[self._fill] = p
             self._fill += 1
             self._state[p] = _IN
@@ -99,5 +124,7 @@ class PageAllocator:
         stale = [p for p in range(1, self.num_pages + 1) if self._state[p] == _LEAVING]
         if stale:
             raise AssertionError(f"pages left half-freed: {stale}")
+        if any(n < 1 or not self.holds(p) for p, n in self._more.items()):
+            raise AssertionError("a page that is in has holders")
         if out + self._fill != self.num_pages:
             raise AssertionError("a page was lost: neither in the stack nor out")

@@ -18,6 +18,10 @@ all layers, host-side lengths, and assign / release / move_row.  What is added h
   the request's row in `[max_rows, *shape]`, is zeroed on `assign`, and moves with
   `move_row`.
 
+* **Forks.**  `fork(src, dst, length)` opens a row as a copy of the first tokens of another one: whole pages are
+  shared (the allocator counts their holders), the page in which the copy ends, which both rows will go on writing, is
+  copied.  Rows that share pages are a family; `families` says which rows of a step share how many keys.
+
 Everything a scheduler decides (which pages a row owns, how long it is) lives on the
 host; `flush()` copies the table rows that changed to the device between steps.
 """
@@ -111,6 +115,7 @@ class PageGroup:
         self.row_pages: List[List[int]] = [[] for _ in range(max_rows)]
         self.freed_upto: List[int] = [0] * max_rows     # blocks below this were given back (window)
         self.dirty: set[int] = set()
+        self.copies: Dict[int, int] = {}                # page -> the page it is to become a copy of (see flush)
 
     def slot_of(self, entry: int) -> int:
         return self.entries.index(entry)
@@ -164,6 +169,12 @@ class CacheManager:
             if specs:
                 self.states[i] = {name: torch.zeros((max_rows, *s.shape), dtype=s.dtype, device=self.device)
                                   for name, s in specs.items()}
+        # Rows that share pages: the family's number (0: none) and how many tokens' pages each shares with all of it.
+        self.family: List[int] = [0] * max_rows
+        self.shared_len: List[int] = [0] * max_rows
+        self._families = 0
+        # The tokens of every row, for sampling that looks at them; None until somebody asks (see keep_tokens)
+        self.tokens: Optional[torch.Tensor] = None
         self._staging: List[Tuple[torch.Tensor, Optional[torch.cuda.Event]]] = []
         self._staging_next = 0
 
@@ -263,7 +274,7 @@ class CacheManager:
             gone = [b for b in range(max(g.freed_upto[row], g.kept_blocks()), upto) if have[b] != 0]
             g.freed_upto[row] = max(g.freed_upto[row], upto)
             if gone:
-                g.allocator.free([have[b] for b in gone])
+                self._give_back(g, [have[b] for b in gone])
                 for b in gone:
                     have[b] = 0
                     g.host_table[row, b] = 0
@@ -276,7 +287,7 @@ class CacheManager:
         for g in self.groups:
             owned = g.owned(row)
             if owned:
-                g.allocator.free(owned)
+                self._give_back(g, owned)
             if g.row_pages[row]:
                 g.host_table[row].zero_()
                 g.dirty.add(row)
@@ -284,6 +295,112 @@ class CacheManager:
             g.freed_upto[row] = 0
         self.lengths[row] = 0
         self.active[row] = False
+        self.family[row] = self.shared_len[row] = 0
+
+    # ------------------------------------------------------------------ forks
+    @staticmethod
+    def _give_back(g: PageGroup, pages: List[int]) -> None:
+        """Free pages of a group; a copy that has not been made yet into a page that nobody holds any more is not made."""
+        g.allocator.free(pages)
+        for p in pages:
+            if p in g.copies and not g.allocator.holds(p):
+                del g.copies[p]
+
+    def _needed_blocks(self, g: PageGroup, length: int) -> List[int]:
+        """Blocks of the first `length` tokens that a query at `length` or later can see."""
+        first, kept = g.first_needed_block(length), g.kept_blocks()
+        return [b for b in range(pages_for(length, self.page_size)) if b >= first or b < kept]
+
+    def can_fork(self, src: int, length: int) -> bool:
+        """Whether row `src` still holds what a row of its first `length` tokens needs: every page that later queries see, and
+        (state slots hold the state after the row's last token alone) no state unless `length` is all of the row."""
+        if not self.active[src] or not 0 < length <= self.lengths[src]:
+            return False
+        if self.states and length != self.lengths[src]:
+            return False
+        return all(b < len(g.row_pages[src]) and g.row_pages[src][b] != 0
+                   for g in self.groups for b in self._needed_blocks(g, length))
+
+    def fork(self, src: int, dst: int, length: int) -> bool:
+        """Open the empty row `dst` as a copy of the first `length` tokens of `src`.  Whole pages get one more holder; the
+        page in which the copy ends is copied (by the next `flush`, on the stream of the step that needs it).
+        Returns False and changes nothing if any group lacks a free page for that."""
+        if self.active[dst]:
+            raise ValueError(f"row {dst} is still in use")
+        if not self.can_fork(src, length):
+            raise ValueError(f"row {src} does not hold its first {length} tokens")
+        whole, rest = divmod(length, self.page_size)
+        if rest and any(g.allocator.n_free < 1 for g in self.groups):
+            return False
+        for g in self.groups:
+            have, needed = g.row_pages[src], set(self._needed_blocks(g, length))
+            pages = [have[b] if b in needed else 0 for b in range(whole)]
+            g.allocator.share([p for p in pages if p])
+            if rest:
+                page = g.allocator.alloc(1)[0]
+                if page in g.copies.values():              # a copy out of it waits: first that one
+                    self._copy(g)
+                g.copies[page] = g.copies.get(have[whole], have[whole])
+                pages.append(page)
+            g.row_pages[dst] = pages
+            g.freed_upto[dst] = 0
+            g.host_table[dst].zero_()
+            g.host_table[dst, :len(pages)] = torch.tensor(pages, dtype=torch.int32)
+            g.dirty.add(dst)
+        for t in self._state_tensors():
+            t[dst].copy_(t[src])
+        if self.tokens is not None:
+            self.tokens[dst, :length].copy_(self.tokens[src, :length])
+        self.active[dst] = True
+        self.lengths[dst] = length
+        shared = whole * self.page_size
+        if not self.family[src]:
+            self._families += 1
+            self.family[src], self.shared_len[src] = self._families, shared
+        self.family[dst], self.shared_len[dst] = self.family[src], min(shared, self.shared_len[src])
+        return True
+
+    def families(self, rows: Sequence[int]) -> Tuple[List[int], List[int], List[int]]:
+        """Which of `rows` share how many keys: (members, starts, lengths).  Group g is the rows[i] for i in
+        members[starts[g]:starts[g + 1]], which share the pages of their first lengths[g] tokens in every group that gives
+        no pages back; a row that shares with none of the others is a group of its own with length 0."""
+        by_family: Dict[int, List[int]] = {}
+        alone: List[int] = []
+        for i, row in enumerate(rows):
+            if self.shared_len[row] > 0:
+                by_family.setdefault(self.family[row], []).append(i)
+            else:
+                alone.append(i)
+        members, starts, lengths = [], [0], []
+        for several in by_family.values():
+            members += several
+            starts.append(len(members))
+            lengths.append(min(self.shared_len[rows[i]] for i in several) if len(several) > 1 else 0)
+        for i in alone:
+            members.append(i)
+            starts.append(len(members))
+            lengths.append(0)
+        return members, starts, lengths
+
+    def keep_tokens(self) -> torch.Tensor:
+        """The rows' tokens on the device, int32 [max_rows, max_len], from now on (see ops.note_tokens).  Rows that are open
+        already have no tokens there."""
+        if self.tokens is None:
+            self.tokens = torch.zeros((self.max_rows, self.max_len), dtype=torch.int32, device=self.device)
+        return self.tokens
+
+    def _copy(self, g: PageGroup) -> None:
+        """Make the copies of pages that wait."""
+        if not g.copies:
+            return
+        dst, src = list(g.copies), list(g.copies.values())
+        g.copies = {}
+        if self.device.type == "cuda":
+            from ..kernels import ops
+            ops.copy_pages(g.k, g.v, src, dst)
+        else:
+            for pool in (g.k, g.v):
+                pool[:, dst] = pool[:, src]
 
     def move_row(self, src: int, dst: int) -> None:
         """Relocate a live row; only its table row and state slot move, never the pages
@@ -302,6 +419,10 @@ class CacheManager:
             g.dirty.update((src, dst))
         for t in self._state_tensors():
             t[dst].copy_(t[src])
+        if self.tokens is not None:
+            self.tokens[dst].copy_(self.tokens[src])
+        for of in (self.family, self.shared_len):
+            of[dst], of[src] = of[src], 0
         self.lengths[dst], self.lengths[src] = self.lengths[src], 0
         self.active[dst], self.active[src] = True, False
 
@@ -322,8 +443,10 @@ class CacheManager:
         return slot[0]
 
     def flush(self) -> None:
-        """Copy the table rows that changed since the last flush to the device, on the
-        current stream.  Call between steps, before the step that uses them."""
+        """Make the copies of pages that forks left to do, and copy the table rows that changed since the last flush to
+        the device, on the current stream.  Call between steps, before the step that uses them."""
+        for g in self.groups:
+            self._copy(g)
         total = sum(len(g.dirty) for g in self.groups)
         if total == 0:
             return
@@ -364,9 +487,21 @@ class CacheManager:
                     want = have[b] if b < len(have) else 0
                     if int(g.host_table[row, b]) != want:
                         raise AssertionError(f"table of row {row} block {b} disagrees with ownership")
-            if len(owned) != len(set(owned)):
-                raise AssertionError("a page is held by two rows")
+            held: Dict[int, int] = {}
+            for p in owned:
+                held[p] = held.get(p, 0) + 1
+            if any(n != g.allocator.holders(p) for p, n in held.items()):
+                raise AssertionError("a page is held by more or fewer rows than the allocator counts")
+            owned = list(held)
+            if not set(g.copies) <= set(owned):
+                raise AssertionError("a copy waits into a page that no row holds")
             if len(owned) != g.allocator.n_used or not all(g.allocator.holds(p) for p in owned):
                 raise AssertionError("pages owned by rows differ from pages marked used")
             if PageAllocator.NULL in owned:
                 raise AssertionError("the null page is owned")
+            for a in range(self.max_rows):
+                for b in range(a):
+                    if self.family[a] and self.family[a] == self.family[b] and not g.spec.bounded:
+                        n = min(self.shared_len[a], self.shared_len[b]) // self.page_size
+                        if g.row_pages[a][:n] != g.row_pages[b][:n]:
+                            raise AssertionError(f"rows {a} and {b} of one family do not share their first {n} pages")

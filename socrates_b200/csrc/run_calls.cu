@@ -32,6 +32,9 @@ int sb_attention_balanced(void*, float*, float*, int*, const void*, const void*,
                           const int*, const int*, int, int, int, int, int, int, float, int, cudaStream_t);
 int sb_attention_decode_mma(void*, float*, float*, const void*, const void*, const void*, const int*, int, const int*,
                             const int*, int, int, int, int, int, int, float, int, int, float, const float*, int, cudaStream_t);
+int sb_attention_shared(void*, float*, long long, int*, long long, const void*, const void*, const void*, int, const int*, int,
+                        const int*, const int*, const int*, int, const int*, const int*, int, int, int, int, int, int, int, float,
+                        int, int*, cudaStream_t);
 int sb_attention_decode_stream(void*, float*, float*, int*, const void*, const void*, const void*, const int*, int, const int*,
                                const int*, int, int, int, int, int, int, float, int, int, int, cudaStream_t);
 }
@@ -56,7 +59,8 @@ template <typename... Args> constexpr int arity(int (*)(Args...)) { return (int)
 #define SB_ENTRIES(X)                                                                                              \
     X(0, sb_add_rmsnorm) X(1, sb_gemm_tcgen05) X(2, sb_gemm_simt) X(3, sb_qk_norm_rope_kvwrite) X(4, sb_silu_mul)   \
     X(5, sb_attention_simt) X(6, sb_attention_prefill_tcgen05) X(7, sb_attention_prefill_mma)                       \
-    X(8, sb_attention_balanced) X(9, sb_attention_decode_mma) X(10, sb_attention_decode_stream)
+    X(8, sb_attention_balanced) X(9, sb_attention_decode_mma) X(10, sb_attention_decode_stream) \
+    X(11, sb_attention_shared)
 
 // Words that entry point `id` takes, or -1 (host only).
 extern "C" int sb_run_calls_arity(int id) {

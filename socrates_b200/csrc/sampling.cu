@@ -431,6 +431,19 @@ sample_adjusted_kernel(int* __restrict__ out, const float* __restrict__ logits, 
     merge_slices(out, mine, mine + 2 * slices, m, slices, best, best_i, s_val, s_idx, &s_last);
 }
 
+__global__ void note_tokens_kernel(int* __restrict__ history, int rows, int width, const int* __restrict__ ids,
+                                   const int* __restrict__ token_rows, const int* __restrict__ positions, int N,
+                                   const int* __restrict__ feedback, int samples) {
+    sb::pdl_launch_dependents();
+    sb::pdl_wait();
+    const int n = blockIdx.x * blockDim.x + threadIdx.x;
+    if (n >= N) return;
+    const int r = token_rows[n], p = positions[n];
+    int id = ids[n];
+    if (id < 0 && -1 - id < samples) id = feedback[-1 - id];
+    if (r >= 0 && r < rows && p >= 0 && p < width) history[(size_t)r * width + p] = id;
+}
+
 }  // namespace
 
 // How many slices a row of V logits is cut into (so callers can size `scratch`).
@@ -497,5 +510,15 @@ extern "C" int sb_sample_adjusted(int* out, const float* logits, const float* te
     const int smem = per * 4 * (1 + (penalties != nullptr || bias_starts != nullptr));
     sb::launch(sample_adjusted_kernel, dim3(M, slices), dim3(512), smem, stream, out, logits, temperature, seeds, counters, V, per,
                scratch + scratch_ints, a);
+    SB_LAUNCH_CHECK();
+}
+
+// history [rows, width]: token n to place positions[n] of row token_rows[n]; an id -1 - j stands for feedback[j] (null: for nothing).
+extern "C" int sb_note_tokens(int* history, int rows, int width, const int* ids, const int* token_rows, const int* positions, int N,
+                              const int* feedback, int samples, cudaStream_t stream) {
+    SB_REQUIRE(N >= 0 && rows > 0 && width > 0 && samples >= 0, "note_tokens: bad sizes (%d tokens, history of %d x %d)", N, rows, width);
+    if (N == 0) return 0;
+    sb::launch(note_tokens_kernel, dim3((N + 255) / 256), dim3(256), 0, stream, history, rows, width, ids, token_rows, positions, N,
+               feedback, feedback != nullptr ? samples : 0);
     SB_LAUNCH_CHECK();
 }

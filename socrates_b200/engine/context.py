@@ -112,7 +112,7 @@ class StepContext:
                  token_ids, positions, token_rows, seq_starts, seq_rows, seq_first_pos, logit_index,
                  all_decode: bool, max_context: int, host_batch=None, num_sms: int = 148,
                  status: Optional[torch.Tensor] = None, token_feedback: Optional[torch.Tensor] = None,
-                 share_keys: bool = False):
+                 share_keys: bool = False, families=None):
         self.dtype, self.device, self.buffers = dtype, device, buffers
         self.num_tokens, self.num_seqs = num_tokens, num_seqs
         self.token_ids, self.positions, self.token_rows = token_ids, positions, token_rows
@@ -122,6 +122,9 @@ class StepContext:
         self.max_context = max_context      # upper bound of any request's length after this step
         self.host_batch = host_batch        # the host-side entries; None while a graph is recorded
         self.share_keys = share_keys        # a decode step whose rows differ much (see Model.prefers_shares)
+        # (members, starts, lengths) of the requests of one token whose rows share keys (see ops.attention_shared), int32 on the
+        # device; None: not worth its launches, or nobody shares
+        self.families = families
         # keys of the longest request that brings one token (0: there is none, or the step is being recorded)
         self.longest_single = max((e.start + 1 for e in host_batch or () if len(e.tokens) == 1), default=0)
         self.num_sms = num_sms

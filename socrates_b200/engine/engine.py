@@ -23,12 +23,14 @@ import torch
 from ..cache import CacheManager
 from ..config import EngineConfig, load_config
 from ..kernels import require_kernels
-from ..sampling import SamplingParams
+from ..sampling import SamplingParams, pack_allowed
 from ..weights import load_weights, random_tensors_on_device
 from .model import Model
-from .runner import ModelRunner, SamplingArgs, StepEntry
+from .runner import Adjust, ModelRunner, SamplingArgs, StepEntry
 from .tokenizer import encode_prompt
 from .scheduler import PlannedEntry, QueueFull, Request, Scheduler, StepPlan, TooLong
+
+MOST_ADJUSTED = 262144           # tokens of a vocabulary whose logits can be adjusted (see ops.sample_adjusted)
 
 _DTYPES = {"bfloat16": torch.bfloat16, "bf16": torch.bfloat16, "float32": torch.float32,
            "fp32": torch.float32, torch.bfloat16: torch.bfloat16, torch.float32: torch.float32}
@@ -125,11 +127,22 @@ class Engine:
 
     # ------------------------------------------------------------------ requests
     def submit(self, prompt: Union[str, Sequence[int]], max_new_tokens: Optional[int] = None,
-               temperature: float = 0.0, seed: int = 0, stream: bool = False) -> Request:
+               temperature: float = 0.0, seed: int = 0, stream: bool = False, **sampling) -> Request:
         """Queue a prompt (token ids, or text if the engine has a tokenizer).
         Raises QueueFull or TooLong as the reference does (model/inference_paged.py:132-148).
         `stream`: the request gets a thread-safe queue `req.stream` that receives each token as
-        it is produced and None at the end (the reference's `stream` flag, :132-138)."""
+        it is produced and None at the end (the reference's `stream` flag, :132-138).
+        `sampling`: the other fields of SamplingParams (repetition_penalty, presence_penalty, frequency_penalty,
+        logit_bias, allowed)."""
+        return self.submit_answers(prompt, 1, max_new_tokens, temperature, seed, stream, **sampling)[0]
+
+    def submit_answers(self, prompt: Union[str, Sequence[int]], n: int, max_new_tokens: Optional[int] = None,
+                       temperature: float = 0.0, seed: int = 0, stream: bool = False, **sampling) -> List[Request]:
+        """Queue `n` requests for one prompt; answer i samples with seed + i.  One of them computes the prompt and the others
+        go on from its pages (see Scheduler), which their attention reads once for all of them where that pays.  Takes
+        all or, where the queue has no place for so many, none."""
+        if n < 1:
+            raise ValueError(f"{n} answers")
         text = None
         if isinstance(prompt, str):
             if self.tok is None:
@@ -142,12 +155,31 @@ class Engine:
         for t in ids:
             if not 0 <= t < vocab:
                 raise ValueError(f"token id {t} is outside the vocabulary of {vocab}")
-        req = Request(ids=ids, max_new_tokens=max_new_tokens or self.max_new_tokens,
-                      sampling=SamplingParams(float(temperature), int(seed)), prompt=text)
-        if stream:
-            import queue
-            req.stream = queue.Queue()
-        return self.scheduler.submit(req)
+        allowed = sampling.get("allowed")
+        if allowed is not None and not callable(allowed):
+            sampling["allowed"] = allowed = list(allowed)    # an iterator is walked more than once
+        params = [SamplingParams(float(temperature), int(seed) + i, **sampling) for i in range(n)]
+        params[0].validate(vocab)
+        if params[0].adjusts:
+            if vocab > MOST_ADJUSTED:
+                raise ValueError(f"logits of {vocab} tokens cannot be adjusted (at most {MOST_ADJUSTED})")
+            if params[0].penalizes:
+                self.cache.keep_tokens()    # from the prompt's first token on
+        if len(self.scheduler.pending) + n > self.scheduler.max_queue:
+            raise QueueFull(f"{len(self.scheduler.pending)} requests already waiting, {n} more")
+        mask = pack_allowed(allowed, vocab) if allowed is not None and not callable(allowed) else None
+        reqs = []
+        for p in params:
+            req = Request(ids=ids, max_new_tokens=max_new_tokens or self.max_new_tokens, sampling=p, prompt=text)
+            req.mask = mask
+            if stream:
+                import queue
+                req.stream = queue.Queue()
+            reqs.append(self.scheduler.submit(req))
+        if n > 1:
+            for req in reqs:
+                req.siblings = reqs
+        return reqs
 
     # ------------------------------------------------------------------ stepping
     def _launch(self, plan):
@@ -156,8 +188,22 @@ class Engine:
                              e.start, [e.count - 1] if e.samples else [])
                    for e in plan.entries]
         args = [SamplingArgs(t, s, c) for (t, s, c) in self.scheduler.sampling_args(plan)]
+        for a, e in zip(args, (e for e in plan.entries if e.samples)):
+            a.adjust = self._adjust(e.request, e.row, e.start + e.count)
         result = self.runner.step(entries, args)
         return self.runner.begin_read(len(args)) if result.tokens is not None else None
+
+    def _adjust(self, req: Request, row: int, length: int) -> Optional[Adjust]:
+        """How the logits behind the first `length` tokens of `req` are adjusted (None: not at all)."""
+        p = req.sampling
+        if not p.adjusts:
+            return None
+        mask = req.mask
+        if callable(p.allowed):
+            allowed = p.allowed(list(req.output))
+            mask = None if allowed is None else pack_allowed(allowed, self.model.plan.vocab_size)
+            req.exhausted = allowed is not None and mask is None
+        return Adjust(p, row, len(req.ids), length, mask)
 
     def _foresee(self, plan):
         """The plan of the step after `plan`, if it can be known before `plan`'s tokens are:
@@ -176,6 +222,8 @@ class Engine:
             req = e.request
             if e.count != 1 or not e.samples or len(req.output) + 1 >= req.max_new_tokens:
                 return None
+            if callable(req.sampling.allowed):
+                return None                 # what may come next depends on the token that is not there yet
             if e.start + 2 > self.max_len or not self.cache.reserve(e.row, e.start + 2):
                 return None
             entries.append((req, e.row, e.start + 1))
@@ -207,8 +255,8 @@ class Engine:
         if guess is not None:
             early_plan = StepPlan([PlannedEntry(req, row, start, 1, True) for (req, row, start) in guess], [])
             # sampling counters are those the scheduler will name once this step's tokens are recorded
-            args = [SamplingArgs(req.sampling.temperature, req.sampling.seed, len(req.output) + 1)
-                    for (req, _, _) in guess]
+            args = [SamplingArgs(req.sampling.temperature, req.sampling.seed, len(req.output) + 1, self._adjust(req, row, start + 1))
+                    for (req, row, start) in guess]
             entries = [StepEntry(row, [-1 - j], start, [0]) for j, (_, row, start) in enumerate(guess)]
             self.runner.step(entries, args, ahead=1)
             early = (early_plan, self.runner.begin_read(len(args)), args)
@@ -235,7 +283,7 @@ class Engine:
             if a.request is not b.request or a.row != b.row or a.start != b.start or a.count != 1 or not a.samples:
                 return False
         now = self.scheduler.sampling_args(plan)
-        return all((x.temperature, x.seed, x.counter) == tuple(y) for x, y in zip(early_args, now))
+        return all((x.temperature, x.seed, x.counter) == tuple(y) for x, y in zip(early_args, now))      # (adjustments follow)
 
     def run(self) -> None:
         """Until every submitted request is finished (model/inference_paged.py:231-237)."""
@@ -245,12 +293,17 @@ class Engine:
                     raise RuntimeError("the scheduler has requests but could plan no step")
 
     def generate(self, prompts: Sequence[Union[str, Sequence[int]]], max_new_tokens: Optional[int] = None,
-                 temperature: float = 0.0, seed: int = 0) -> List[List[int]]:
+                 temperature: float = 0.0, seed: int = 0, n: int = 1, **sampling):
         """Submit, run, and return the generated ids of each prompt, in order.
-        Request i samples with seed + i."""
-        reqs = [self.submit(p, max_new_tokens, temperature, seed + i) for i, p in enumerate(prompts)]
+        Request i samples with seed + i.  `n` > 1: so many answers a prompt, a list of lists each; answer j of prompt i
+        samples with seed + i * n + j.  `sampling`: as in `submit`."""
+        if n == 1:
+            reqs = [self.submit(p, max_new_tokens, temperature, seed + i, **sampling) for i, p in enumerate(prompts)]
+            self.run()
+            return [r.output for r in reqs]
+        answers = [self.submit_answers(p, n, max_new_tokens, temperature, seed + i * n, **sampling) for i, p in enumerate(prompts)]
         self.run()
-        return [r.output for r in reqs]
+        return [[r.output for r in reqs] for reqs in answers]
 
 
 __all__ = ["Engine", "Request", "QueueFull", "TooLong", "build_model", "build_random_model",

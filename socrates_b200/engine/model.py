@@ -47,6 +47,7 @@ class Model:
                 if hasattr(p, "prefers_shares"):
                     dealers.setdefault((p.Hq, p.Hkv, p.D, p.window), p)
         self._key_dealers = list(dealers.values())
+        self._family_readers = [p for p in self._key_dealers if hasattr(p, "prefers_families")]
         # layers of equal specs that run after each order entry: a recording pays from the second on (the last layer's
         # products are followed by another matrix).  Whether layers are alike is for _like_another to see.
         kinds: List = []
@@ -113,6 +114,11 @@ class Model:
         """Whether a decode step over rows of so many keys should deal the keys of all rows to the GPU's blocks in equal
         shares (parts say so through an optional `prefers_shares`; asked once for layers of one shape)."""
         return any(p.prefers_shares(lengths, num_sms) for p in self._key_dealers)
+
+    def prefers_families(self, shared) -> bool:
+        """Whether a step with families of (rows, shared keys) should read shared keys once (parts say so through an
+        optional `prefers_families`)."""
+        return any(p.prefers_families(shared) for p in self._family_readers)
 
     # ------------------------------------------------------------------ one step
     def _like_another(self, ctx: StepContext, stream: ResidualStream, view: CacheView, i: int,

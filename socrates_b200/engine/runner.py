@@ -23,6 +23,7 @@ import torch
 from ..cache.manager import CacheManager
 from ..kernels import ops
 from ..kernels.library import Counters
+from ..sampling import MAX_BIASES, SamplingParams
 from .context import Buffers, StepContext
 from .model import Model
 
@@ -43,6 +44,19 @@ class SamplingArgs:
     temperature: float = 0.0
     seed: int = 0
     counter: int = 0
+    adjust: Optional["Adjust"] = None       # what happens to the logits first
+
+
+@dataclass
+class Adjust:
+    """How the logits of one wanted row are adjusted (see ops.sample_adjusted): the penalties and biases of `params`, over
+    the tokens that the cache keeps of `row` (CacheManager.keep_tokens) with this step's, of which the first `prompt_len`
+    are the prompt; `mask`: which tokens are allowed (sampling.pack_allowed), None for all."""
+    params: SamplingParams
+    row: int
+    prompt_len: int
+    length: int
+    mask: Optional[object] = None
 
 
 @dataclass
@@ -62,7 +76,75 @@ class _Layout:
         self.seq_starts = 7 * T
         self.seq_rows = self.seq_starts + R + 1
         self.seq_first = self.seq_rows + R
-        self.total = self.seq_first + R
+        # requests of one token whose rows share keys: members, their groups' starts, shared lengths
+        self.members = self.seq_first + R
+        self.starts = self.members + R
+        self.shared = self.starts + R + 1
+        self.total = self.shared + R
+
+
+class _Adjustments:
+    """The arrays that sample_adjusted takes beside the step's, on the device and pinned; made when the first request that
+    adjusts its logits is sampled."""
+
+    def __init__(self, rows: int, vocab: int, device):
+        self.rows, self.device = rows, device
+        # int32 words: cache rows, prompt lengths, lengths, mask rows, penalties (float32 [rows, 3]), starts, ids, values
+        sizes = (rows, rows, rows, rows, 3 * rows, rows + 1, rows * MAX_BIASES, rows * MAX_BIASES)
+        self.at = [sum(sizes[:i]) for i in range(len(sizes) + 1)]
+        self.small = self.at[6]             # words that every step copies; biases and masks only where there are any
+        self.dev = torch.zeros(self.at[-1], dtype=torch.int32, device=device)
+        self.mask = torch.zeros((rows, -(-vocab // 32)), dtype=torch.int32, device=device)
+        self.host = [[torch.zeros(self.at[-1], dtype=torch.int32).pin_memory(),
+                      torch.zeros(self.mask.shape, dtype=torch.int32).pin_memory(), None] for _ in range(4)]
+        self.next = 0
+
+    def fill(self, args: Sequence[Optional["Adjust"]]) -> None:
+        slot = self.host[self.next]
+        self.next = (self.next + 1) % len(self.host)
+        buf, masks, event = slot
+        if event is not None:
+            event.synchronize()
+        at, words = self.at, buf.numpy()
+        floats = buf.view(torch.float32).numpy()
+        n = masked = 0
+        for m, a in enumerate(args):
+            p = a.params if a is not None else None
+            penal = p is not None and p.penalizes
+            words[at[0] + m] = a.row if penal else 0
+            words[at[1] + m] = a.prompt_len if penal else 0
+            words[at[2] + m] = a.length if penal else 0
+            floats[at[4] + 3 * m:at[4] + 3 * m + 3] = ((p.repetition_penalty, p.presence_penalty, p.frequency_penalty) if penal
+                                                       else (1.0, 0.0, 0.0))
+            words[at[3] + m] = -1
+            if a is not None and a.mask is not None:
+                words[at[3] + m] = masked
+                masks[masked].numpy()[:] = a.mask
+                masked += 1
+            words[at[5] + m] = n
+            if p is not None and p.logit_bias:
+                k = len(p.logit_bias)
+                words[at[6] + n:at[6] + n + k] = [int(t) for t in p.logit_bias]
+                floats[at[7] + n:at[7] + n + k] = list(p.logit_bias.values())
+                n += k
+        words[at[5] + len(args)] = n
+        self.dev[:self.small].copy_(buf[:self.small], non_blocking=True)
+        if n:
+            for i in (6, 7):
+                self.dev[at[i]:at[i] + n].copy_(buf[at[i]:at[i] + n], non_blocking=True)
+        if masked:
+            self.mask[:masked].copy_(masks[:masked], non_blocking=True)
+        if event is None:
+            event = slot[2] = torch.cuda.Event()
+        event.record()
+
+    def of(self, M: int) -> dict:
+        """The keyword arguments of sample_adjusted for M rows."""
+        at, d = self.at, self.dev
+        return {"history_rows": d[at[0]:at[0] + M], "prompt_lens": d[at[1]:at[1] + M], "lengths": d[at[2]:at[2] + M],
+                "mask_rows": d[at[3]:at[3] + M], "penalties": d[at[4]:at[4] + 3 * M].view(torch.float32).view(M, 3),
+                "bias_starts": d[at[5]:at[5] + M + 1], "bias_ids": d[at[6]:at[7]], "bias_values": d[at[7]:at[8]].view(torch.float32),
+                "mask": self.mask}
 
 
 class ModelRunner:
@@ -98,14 +180,15 @@ class ModelRunner:
         self.sample_scratch = torch.zeros(ops.sample_scratch_size(max_tokens, self.vocab), dtype=torch.int32,
                                           device=self.device)
         self.use_graphs = use_graphs and model.supports_graph
-        # by (rows, whether tokens are drawn, whether keys are dealt in shares)
-        self._graphs: Dict[Tuple[int, bool, bool], Tuple[torch.cuda.CUDAGraph, Optional[torch.Tensor]]] = {}
+        # by (rows, whether tokens are drawn, whether keys are dealt in shares), and what else the step does
+        self._graphs: Dict[tuple, Tuple[torch.cuda.CUDAGraph, Optional[torch.Tensor]]] = {}
         self._eager_decode_done: set = set()
         self.num_sms = torch.cuda.get_device_properties(self.device).multi_processor_count
         self.steps_run = 0
         self.graph_replays = 0
         self.kernel_launches = 0    # kernels launched by steps, replays of recorded graphs included
-        self._graph_kernels: Dict[Tuple[int, bool, bool], int] = {}
+        self._graph_kernels: Dict[tuple, int] = {}
+        self._adjustments: Optional[_Adjustments] = None
 
     # ------------------------------------------------------------------ staging
     def _stage(self) -> Tuple[torch.Tensor, int]:
@@ -116,7 +199,7 @@ class ModelRunner:
             ev.synchronize()
         return buf, i
 
-    def _fill(self, entries: Sequence[StepEntry], sampling, ahead: int = 0) -> Tuple[int, int, int, bool, int]:
+    def _fill(self, entries: Sequence[StepEntry], sampling, ahead: int = 0, families=None) -> Tuple[int, int, int, bool, int]:
         L = self.layout
         if not entries:
             raise ValueError("a step needs at least one entry")
@@ -180,6 +263,13 @@ class ModelRunner:
         nb[L.seq_starts:L.seq_starts + R + 1] = starts
         nb[L.seq_rows:L.seq_rows + R] = [e.row for e in entries]
         nb[L.seq_first:L.seq_first + R] = [e.start for e in entries]
+        if families is not None:
+            members, family_starts, shared = families
+            groups = len(shared)
+            nb[L.members:L.members + len(members)] = members
+            # as many groups as members, the last ones empty: a recorded graph has one size a width
+            nb[L.starts:L.starts + len(members) + 1] = family_starts + [len(members)] * (len(members) - groups)
+            nb[L.shared:L.shared + len(members)] = shared + [0] * (len(members) - groups)
         self.dev_meta.copy_(buf, non_blocking=True)     # the step's one host-to-device copy
         ev = self._events[slot]
         ev.record()
@@ -187,7 +277,8 @@ class ModelRunner:
         return N, M, R, all_decode, max_ctx
 
     def _context(self, N: int, M: int, R: int, all_decode: bool, max_ctx: int, host_batch,
-                 share_keys: bool = False) -> StepContext:
+                 share_keys: bool = False, members: int = 0) -> StepContext:
+        """`members`: requests of one token in the families that were filled in (0: none)."""
         L, m = self.layout, self.dev_meta
         return StepContext(
             self.dtype, self.device, self.buffers, N, R,
@@ -196,7 +287,9 @@ class ModelRunner:
             seq_first_pos=m[L.seq_first:L.seq_first + R],
             logit_index=m[L.logit:L.logit + M] if M else None,
             all_decode=all_decode, max_context=max_ctx, host_batch=host_batch, num_sms=self.num_sms,
-            status=self.status, token_feedback=self.sampled, share_keys=share_keys)
+            status=self.status, token_feedback=self.sampled, share_keys=share_keys,
+            families=(m[L.members:L.members + members], m[L.starts:L.starts + members + 1],
+                      m[L.shared:L.shared + members]) if members else None)
 
     def begin_read(self, count: int) -> Tuple[int, int]:
         """Start the copy of the `count` tokens the last step sampled (and of the kernels'
@@ -277,16 +370,38 @@ class ModelRunner:
             raise RuntimeError(f"a tensor-core kernel gave up waiting on its pipeline (code {code}); "
                                f"the step's results are not valid")
 
-    def _run(self, ctx: StepContext, M: int, sample: bool):
+    def _run(self, ctx: StepContext, M: int, sample: bool, adjust: bool = False):
         with ops.stream_scope():            # one stream look-up for the step's kernels (also while a graph records)
             logits = self.model.forward(ctx, self.cache)
             tokens = None
+            if self.cache.tokens is not None:       # before the sampler writes over what ids may stand for
+                ops.note_tokens(self.cache.tokens, ctx.token_ids, ctx.token_rows, ctx.positions, self.sampled)
             if sample and M:
                 L, m = self.layout, self.dev_meta
                 tokens = self.sampled[:M]
-                ops.sample(tokens, logits, m[L.temp:L.temp + M].view(torch.float32),
-                           m[L.seed:L.seed + M], m[L.counter:L.counter + M], self.sample_scratch)
+                args = (tokens, logits, m[L.temp:L.temp + M].view(torch.float32), m[L.seed:L.seed + M],
+                        m[L.counter:L.counter + M], self.sample_scratch)
+                if adjust:
+                    ops.sample_adjusted(*args, history=self.cache.tokens, **self._adjustments.of(M))
+                else:
+                    ops.sample(*args)
         return logits, tokens
+
+    def _families(self, entries: Sequence[StepEntry]):
+        """(members, starts, shared lengths) of the entries of one token whose rows share keys, if reading those keys once
+        pays, else None.  Members are tokens of the step."""
+        if self.dtype != torch.bfloat16 or not any(self.cache.shared_len):
+            return None
+        tokens, rows, n = [], [], 0
+        for e in entries:
+            if len(e.tokens) == 1:
+                tokens.append(n)
+                rows.append(e.row)
+            n += len(e.tokens)
+        members, starts, shared = self.cache.families(rows)
+        if not self.model.prefers_families([(b - a, k) for a, b, k in zip(starts, starts[1:], shared)]):
+            return None
+        return [tokens[i] for i in members], starts, shared
 
     def prepare(self, entries: Sequence[StepEntry],
                 sampling: Optional[Sequence[SamplingArgs]] = None) -> StepContext:
@@ -306,20 +421,29 @@ class ModelRunner:
         starts one past its row's committed length (and may name its token as -1 - j, the j-th
         token the step before sampled)."""
         self.cache.flush()
-        N, M, R, all_decode, max_ctx = self._fill(entries, sampling, ahead)
+        families = self._families(entries)
+        N, M, R, all_decode, max_ctx = self._fill(entries, sampling, ahead, families)
+        members = len(families[0]) if families is not None else 0
         sample = sampling is not None
+        adjust = sample and any(a.adjust is not None for a in sampling)
+        if adjust:
+            if self._adjustments is None:
+                self.cache.keep_tokens()
+                self._adjustments = _Adjustments(self.max_wanted, self.vocab, self.device)
+            self._adjustments.fill([a.adjust for a in sampling])
         # decoding rows of very different lengths go through another attention kernel (and a graph of their own)
-        share = (all_decode and self.dtype == torch.bfloat16
+        share = (all_decode and not members and self.dtype == torch.bfloat16
                  and self.model.prefers_shares([e.start + 1 for e in entries], self.num_sms))
         self.steps_run += 1
         if self.use_graphs and all_decode and M == N:
             key = (N, sample, share)
+            key += tuple(name for name, on in (("families", members), ("tokens", self.cache.tokens is not None), ("adjust", adjust)) if on)
             if key not in self._graphs and key in self._eager_decode_done:
-                ctx = self._context(N, M, R, True, self.cache.max_len, None, share)
+                ctx = self._context(N, M, R, True, self.cache.max_len, None, share, members)
                 graph = torch.cuda.CUDAGraph()
                 before = Counters.launches
                 with torch.cuda.graph(graph):
-                    logits, tokens = self._run(ctx, M, sample)
+                    logits, tokens = self._run(ctx, M, sample, adjust)
                 self._graph_kernels[key] = Counters.launches - before
                 self._graphs[key] = (graph, logits, tokens)
             if key in self._graphs:
@@ -330,9 +454,9 @@ class ModelRunner:
                 return StepResult(logits, tokens, N)
             self._eager_decode_done.add(key)
             max_ctx = self.cache.max_len     # the same launch shapes the graph will record
-        ctx = self._context(N, M, R, all_decode, max_ctx, entries, share)
+        ctx = self._context(N, M, R, all_decode, max_ctx, entries, share, members)
         before = Counters.launches
-        logits, tokens = self._run(ctx, M, sample)
+        logits, tokens = self._run(ctx, M, sample, adjust)
         self.kernel_launches += Counters.launches - before
         return StepResult(logits, tokens, N)
 

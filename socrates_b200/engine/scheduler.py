@@ -23,6 +23,10 @@ the cancelled flag, retire + compaction + refill in the same iteration.  Changed
   is itself the most recently admitted, it waits for this step (a prompt portion is
   first shrunk to the pages that are free).  The oldest request can therefore always
   proceed, and `submit` refuses requests that could not fit the pool alone.
+* **Answers of one prompt** (`Request.siblings`).  One of them computes the prompt; the others wait until it has and are
+  admitted as forks of its row, all but the last prompt token shared (`CacheManager.fork`), so each draws its first token
+  from logits of its own step.  Where that is not possible (nobody of them is live, pages behind a window were given
+  back, the layers keep state) they compute the prompt as any request does.
 """
 
 from __future__ import annotations
@@ -46,7 +50,7 @@ class TooLong(Exception):
     """Prompt plus new tokens exceed a row or the page pool (model/inference_paged.py:144-146)."""
 
 
-@dataclass
+@dataclass(eq=False)              # one request is no other, whatever they ask for
 class Request:
     """One generation request; field names follow the reference's Request
     (model/inference_cont.py:65-82) where it has them."""
@@ -67,6 +71,10 @@ class Request:
     # model/inference_paged.py:136-138, 196-198, is an asyncio queue fed from the serve thread; this
     # one is thread-safe and needs no event loop)
     stream: Optional["queue.Queue"] = None
+    # the answers of one prompt, this one among them (see Scheduler); empty: there are no others
+    siblings: List["Request"] = field(default_factory=list, repr=False)
+    mask: Optional[object] = field(default=None, repr=False)      # a fixed set of allowed tokens, packed
+    exhausted: bool = False    # nothing may follow (the request's grammar): the next token drawn ends it
     # scheduler state
     cached: int = 0            # tokens of ids + output that are in the cache
     preemptions: int = 0
@@ -150,12 +158,14 @@ class Scheduler:
         return bool(self.pending) or self.n_active > 0
 
     # ------------------------------------------------------------------ rows
-    def _admit(self, req: Request) -> None:
+    def _admit(self, req: Request, forked: int = 0) -> None:
+        """Give `req` a row: an empty one, or the one that holds its first `forked` tokens already."""
         row = self.n_active
-        self.cache.assign(row)
+        if not forked:
+            self.cache.assign(row)
         self.rows[row] = req
         req.row = row
-        req.cached = 0
+        req.cached = forked
         req.order = self._admissions
         self._admissions += 1
         if not req.admitted:
@@ -245,18 +255,30 @@ class Scheduler:
             elif prefill_budget >= 1:
                 prefill_budget -= self._plan_portion(req, prefill_budget, planned, preempted)
 
-        # admissions, FIFO, while a row and budget are left
-        while self.pending and self.n_active < self.max_batch and prefill_budget >= 1:
-            req = self.pending[0]
+        # admissions, FIFO, while a row and budget are left; answers whose prompt is being computed let others pass
+        at = 0
+        while at < len(self.pending) and self.n_active < self.max_batch and prefill_budget >= 1:
+            req = self.pending[at]
             if req.cancelled:
-                self._drop(self.pending.popleft())
+                del self.pending[at]
+                self._drop(req)
                 continue
-            if req in preempted:
+            if any(req is r for r in preempted):
                 break                       # it just gave up its pages: not in this step
-            if not self._room_to_admit(req, prefill_budget):
+            src = self._sibling(req)
+            if src is not None and src.cached < len(req.ids) - 1:
+                at += 1
+                continue
+            forked = 0
+            if src is not None:
+                if not self._room_to_fork():
+                    break
+                if self.cache.fork(src.row, self.n_active, len(req.ids) - 1):
+                    forked = len(req.ids) - 1
+            if not forked and not self._room_to_admit(req, prefill_budget):
                 break                       # it would only take pages that the live requests need next
-            self.pending.popleft()
-            self._admit(req)
+            del self.pending[at]
+            self._admit(req, forked)
             prefill_budget -= self._plan_portion(req, prefill_budget, planned, preempted)
 
         if not planned:
@@ -265,6 +287,24 @@ class Scheduler:
         for e in planned:
             e.row = e.request.row           # compaction after a preemption may have moved rows
         return StepPlan(planned, preempted)
+
+    def _sibling(self, req: Request) -> Optional[Request]:
+        """A live answer of the same prompt from whose row `req` can be forked, now or when it has computed the prompt."""
+        need = len(req.ids) - 1
+        if need < 1:
+            return None
+        live = [s for s in req.siblings if s is not req and s.row >= 0 and not s.done and not s.cancelled]
+        for s in live:
+            if s.cached >= need and self.cache.can_fork(s.row, need):
+                return s
+        if self.cache.states:               # state after all of the prompt but its last token is never at hand again
+            return None
+        return next((s for s in live if s.cached < need), None)
+
+    def _room_to_fork(self) -> bool:
+        """Whether every group has a page for the end of the prompt, one for what follows, and one to spare for each live
+        request (see _room_to_admit)."""
+        return all(g.allocator.n_free >= min(2 + self.n_active, g.allocator.num_pages) for g in self.cache.groups)
 
     def _room_to_admit(self, req: Request, budget: int) -> bool:
         """Whether admitting `req` now is worth a row.  With nobody live it always is (the oldest
@@ -331,7 +371,7 @@ class Scheduler:
         request and is not appended; so does reaching max_new_tokens."""
         if not req.first_token:
             req.first_token = now
-        if token in self.stop_ids:
+        if token in self.stop_ids or req.exhausted:
             req.done = True
         else:
             req.output.append(token)

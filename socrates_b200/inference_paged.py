@@ -66,6 +66,10 @@ def main(argv=None) -> int:
     ap.add_argument("--num-blocks", type=int, default=None, help="pages in the pool (default: from free memory, at most max_batch rows of max_len)")
     ap.add_argument("--token-budget", type=int, default=2048, help="most tokens one step runs")
     ap.add_argument("--temperature", type=float, default=0.0, help="0 = greedy")
+    ap.add_argument("--answers", type=int, default=1, help="answers a prompt; they share its pages")
+    ap.add_argument("--repetition-penalty", type=float, default=1.0, help="for tokens in the prompt or the answer (1 = none)")
+    ap.add_argument("--presence-penalty", type=float, default=0.0, help="for tokens in the answer")
+    ap.add_argument("--frequency-penalty", type=float, default=0.0, help="for every time a token stands in the answer")
     ap.add_argument("--no-compile", action="store_true", help="no CUDA graphs (same as COMPILE=0)")
     ap.add_argument("--no-warmup", action="store_true",
                     help="record each decode graph at the first step of its width instead of at start-up")
@@ -114,7 +118,11 @@ def main(argv=None) -> int:
         n = args.num_prompts or 4
         prompts += [torch.randint(1, vocab, (args.prompt_len,), generator=g).tolist() for _ in range(n)]
 
-    reqs = [engine.submit(p, temperature=args.temperature, seed=args.seed + i) for i, p in enumerate(prompts)]
+    prompts = [p for p in prompts for _ in range(args.answers)]
+    reqs = [r for i, p in enumerate(prompts[::args.answers])
+            for r in engine.submit_answers(p, args.answers, temperature=args.temperature, seed=args.seed + i * args.answers,
+                                           repetition_penalty=args.repetition_penalty, presence_penalty=args.presence_penalty,
+                                           frequency_penalty=args.frequency_penalty)]
     pages = engine.cache.groups[0].allocator.num_pages if engine.cache.groups else 0
     print(f"{len(reqs)} requests, {engine.max_batch} rows, {pages} blocks of {args.block_size}\n")
     t0 = time.perf_counter()

@@ -25,9 +25,10 @@ from .library import F, P, Counters, KernelError, _SIGNATURES, library, set_reco
 # the entry points that a recorded layer may consist of, by their number in run_calls.cu
 ENTRIES = {"sb_add_rmsnorm": 0, "sb_gemm_tcgen05": 1, "sb_gemm_simt": 2, "sb_qk_norm_rope_kvwrite": 3, "sb_silu_mul": 4,
            "sb_attention_simt": 5, "sb_attention_prefill_tcgen05": 6, "sb_attention_prefill_mma": 7,
-           "sb_attention_balanced": 8, "sb_attention_decode_mma": 9, "sb_attention_decode_stream": 10}
+           "sb_attention_balanced": 8, "sb_attention_decode_mma": 9, "sb_attention_decode_stream": 10,
+           "sb_attention_shared": 11}
 # host-only questions that a layer may ask while it is recorded
-_QUESTIONS = ("_supports", "_splits", "_parts", "_shares", "_kernels", "_blocks_per_sm", "sb_last_error",
+_QUESTIONS = ("_supports", "_splits", "_parts", "_shares", "_kernels", "_scratch", "_blocks_per_sm", "sb_last_error",
               "sb_set_dependent_launch")
 
 

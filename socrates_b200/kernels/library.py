@@ -39,6 +39,7 @@ _SIGNATURES = {
     "sb_sample_slices": [I],
     "sb_sample_adjusted_slices": [I],
     "sb_sample_adjusted": [P, P, P, P, P, I, I, P, LL, P, I, P, P, P, P, P, P, P, P, I, P, P, P],
+    "sb_note_tokens": [P, I, I, P, P, P, I, P, I, P],
     "sb_copy_pages": [P, P, P, P, I, I, I, LL, LL, P],
     "sb_copy_pages_kernels": [I],
     "sb_attention_shared_scratch": [I, I, I, I, I, I, P, P],

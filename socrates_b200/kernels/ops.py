@@ -10,6 +10,7 @@ model/kernels/csrc/ops.cpp:29-72.)
 from __future__ import annotations
 
 import ctypes
+import functools
 from array import array
 from typing import Optional, Sequence, Tuple
 
@@ -323,6 +324,24 @@ def sample_adjusted(out: torch.Tensor, logits: torch.Tensor, temperature: Option
         kernels=1 if M else 0)
 
 
+def note_tokens(history: torch.Tensor, ids: torch.Tensor, rows: torch.Tensor, positions: torch.Tensor,
+                feedback: Optional[torch.Tensor] = None) -> None:
+    """history[rows[n], positions[n]] = ids[n]: what `sample_adjusted` looks at, kept step by step.  history int32
+    [rows, tokens]; ids, rows and positions int32 [N] (places outside `history` are passed over); with `feedback` (int32) an
+    id -1 - j stands for feedback[j], as in `embed`."""
+    if history.dim() != 2:
+        raise KernelError(f"history must be [rows, tokens], got {tuple(history.shape)}")
+    N, i32 = ids.numel(), torch.int32
+    wanted = [(history, "history", i32, None), (ids, "ids", i32, (N,)), (rows, "rows", i32, (N,)), (positions, "positions", i32, (N,))]
+    if feedback is not None:
+        wanted.append((feedback, "feedback", i32, None))
+    _check(torch.cuda.current_device(), wanted)
+    lib = library()
+    check(lib, lib.sb_note_tokens(history.data_ptr(), history.shape[0], history.shape[1], ids.data_ptr(), rows.data_ptr(),
+                                  positions.data_ptr(), N, _ptr(feedback), 0 if feedback is None else feedback.numel(), _stream()),
+          "note_tokens", kernels=1 if N else 0)
+
+
 def copy_pages(k_pools: torch.Tensor, v_pools: torch.Tensor, src: Sequence[int], dst: Sequence[int]) -> None:
     """Copy page src[i] to page dst[i] in every layer run of a cache group: k_pools [runs, pages, Hkv, BS, D] and v_pools
     [runs, pages, Hkv, BS, Dv] of one dtype.
@@ -352,6 +371,7 @@ def copy_pages(k_pools: torch.Tensor, v_pools: torch.Tensor, src: Sequence[int],
                                  value_page, _stream()), "copy_pages", kernels=lib.sb_copy_pages_kernels(n))
 
 
+@functools.lru_cache(maxsize=None)
 def attention_shared_scratch_size(members: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int,
                                   dtype: torch.dtype) -> Tuple[int, int]:
     """(float32, int32) entries of scratch that `attention_shared` needs for up to so many members, in at most as many

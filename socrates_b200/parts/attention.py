@@ -16,7 +16,7 @@ portions and portions of prompts share a step with decode tokens.
 from __future__ import annotations
 
 import os
-from typing import Dict, Mapping, Optional, Sequence
+from typing import Dict, Mapping, Optional, Sequence, Tuple
 
 import torch
 
@@ -68,6 +68,10 @@ def decode_partitions(ctx, num_kv_heads: int, blocks_per_sm: int, keys_per_part:
 SINGLES_APART_FROM = 1024
 
 
+# From so many bytes of keys and values that need not be read again on, shared keys are read once.
+SHARED_PAYS_FROM = 48 << 20
+
+
 def balanced_attention(ctx, out, q, k_pool, v_pool, table, num_heads: int, scale: float, window: int) -> None:
     """The step's requests of one token through the equal-shares decode kernel, with scratch of the step."""
     Hkv, D, R = k_pool.shape[1], k_pool.shape[3], ctx.num_seqs
@@ -78,6 +82,17 @@ def balanced_attention(ctx, out, q, k_pool, v_pool, table, num_heads: int, scale
                                   take("attn_share_o", num_heads * shares * 2 * D, torch.float32),
                                   take("attn_share_ml", num_heads * shares * 2 * 2, torch.float32),
                                   take("attn_share_counters", ctx.buffers.max_rows * Hkv, torch.int32, zeroed=True))
+
+
+def shared_attention(ctx, out, q, k_pool, v_pool, table, num_heads: int, scale: float, window: int) -> None:
+    """The step's requests of one token through the kernels that read the keys of a family once, with scratch of the step."""
+    Hkv, page_size, D = k_pool.shape[1], k_pool.shape[2], k_pool.shape[3]
+    members, starts, lengths = ctx.families
+    floats, ints = ops.attention_shared_scratch_size(members.numel(), num_heads, Hkv, D, page_size, q.dtype)
+    take = ctx.buffers.take_flat
+    ops.attention_shared(out, q, k_pool, v_pool, table, ctx.token_rows, ctx.positions, members, starts, lengths, num_heads, scale,
+                         window, take("attn_shared_part", floats, torch.float32),
+                         take("attn_shared_lists", ints, torch.int32, zeroed=True), ctx.status)
 
 
 def paged_attention(ctx, out, q, k_pool, v_pool, table, num_heads: int, scale: float, window: int,
@@ -96,12 +111,24 @@ def paged_attention(ctx, out, q, k_pool, v_pool, table, num_heads: int, scale: f
     bfloat16, other steps: the tile kernels (tcgen05 for head sizes 64 and 128, mma.sync for 16 and
     32); beside the tcgen05 kernel, decoding requests with long rows in the equal-shares kernel.  Everything else (the float32 engine above all): the SIMT kernel, whose split depends on
     `max_len` of the cache alone, so the float32 engine's numbers never depend on the batch.
+
+    Where the step says so (`ctx.families`: rows that share a prefix long enough, PAGED_PARTITION "auto", bfloat16, no
+    window), the requests of one token go through `shared_attention` instead.
     """
     Hkv, page_size, D = k_pool.shape[1], k_pool.shape[2], k_pool.shape[3]
     N = q.shape[0]
     bf16 = q.dtype == torch.bfloat16
+    shared = bf16 and ctx.families is not None and not window
+    if shared and ctx.all_decode:
+        shared_attention(ctx, out, q, k_pool, v_pool, table, num_heads, scale, window)
+        return
     if bf16 and not ctx.all_decode:
         if ctx.status is not None and ops.attention_tcgen05_supports(num_heads, Hkv, D, page_size):
+            if shared:
+                ops.attention_prefill_tcgen05(out, q, k_pool, v_pool, table, ctx.seq_starts, ctx.seq_rows, ctx.seq_first_pos,
+                                              num_heads, scale, ctx.status, window, skip_single=True, meta_older=True)
+                shared_attention(ctx, out, q, k_pool, v_pool, table, num_heads, scale, window)
+                return
             apart = (paged_partition() is None and ctx.longest_single >= SINGLES_APART_FROM
                      and ops.attention_balanced_supports(num_heads, Hkv, D, page_size, ctx.num_seqs))
             ops.attention_prefill_tcgen05(out, q, k_pool, v_pool, table, ctx.seq_starts, ctx.seq_rows,
@@ -232,6 +259,14 @@ class GQAAttention(Part):
             return longest >= 16
         total = sum(lengths) / 64 + N / 2
         return -(-longest // parts) - total / shares >= 8
+
+    def prefers_families(self, shared: Sequence[Tuple[int, int]]) -> bool:
+        """Whether the requests of one token of a step whose families are `shared`, (rows, shared keys) each, should read shared
+        keys once (attention_shared.cu) rather than every row its own way."""
+        if self.window or paged_partition() is not None:
+            return False
+        saved = sum((n - 1) * keys for n, keys in shared)
+        return saved * self.Hkv * self.D * 4 >= SHARED_PAYS_FROM
 
     def forward(self, ctx, x: torch.Tensor, cache) -> Branch:
         N = x.shape[0]

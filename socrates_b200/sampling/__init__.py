@@ -19,21 +19,82 @@ three-round xorshift-multiply finalizer (constants 0x7FEB352D, 0x846CA68B, shift
 `counter` is the number of tokens the request has produced so far, so a request's
 tokens depend on its seed alone: not on the batch it ran in, not on how its prompt was
 cut, not on whether it was preempted and recomputed.
+
+Before either rule a request may have its logits adjusted (in the same kernel's pass; see kernels/ops.py
+sample_adjusted for the formulas): penalties for tokens that its prompt and output hold already, biases on single
+tokens, and a set of allowed tokens, fixed or (a grammar) a function of the output so far.
 """
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
+from typing import Callable, Iterable, Mapping, Optional, Union
+
+import numpy as np
+
+MAX_BIASES = 512                 # of one request
 
 
 @dataclass(frozen=True)
 class SamplingParams:
     temperature: float = 0.0     # 0 = greedy
     seed: int = 0
+    repetition_penalty: float = 1.0      # logits of tokens in the prompt or output: l / r if l > 0 else l * r
+    presence_penalty: float = 0.0        # taken off logits of tokens in the output
+    frequency_penalty: float = 0.0       # taken off once for every time a token stands in the output
+    logit_bias: Optional[Mapping[int, float]] = None        # token -> what is added to its logit
+    # The tokens that may come next: ids, or a function from the output so far (a list of ids) to ids, to a packed mask
+    # (`pack_allowed`), or to None for all.  A function that allows nothing ends the request.
+    allowed: Optional[Union[Iterable[int], Callable]] = None
 
-    def validate(self) -> None:
+    def validate(self, vocab: Optional[int] = None) -> None:
+        """`vocab`: check token ids, too."""
         if not self.temperature >= 0.0:
             raise ValueError(f"temperature must be >= 0, got {self.temperature}")
+        if not (0.0 < self.repetition_penalty < math.inf):
+            raise ValueError(f"repetition_penalty must be positive, got {self.repetition_penalty}")
+        for name in ("presence_penalty", "frequency_penalty"):
+            if not math.isfinite(getattr(self, name)):
+                raise ValueError(f"{name} must be finite, got {getattr(self, name)}")
+        if self.logit_bias is not None:
+            if len(self.logit_bias) > MAX_BIASES:
+                raise ValueError(f"{len(self.logit_bias)} biases; a request has at most {MAX_BIASES}")
+            for t, b in self.logit_bias.items():
+                if vocab is not None and not 0 <= int(t) < vocab:
+                    raise ValueError(f"a bias on token {t}, outside the vocabulary of {vocab}")
+                if math.isnan(b) or b == math.inf:
+                    raise ValueError(f"a bias of {b} on token {t}")
+        if self.allowed is not None and not callable(self.allowed) and vocab is not None:
+            if pack_allowed(self.allowed, vocab) is None:
+                raise ValueError("no token is allowed")
+
+    @property
+    def penalizes(self) -> bool:
+        return self.repetition_penalty != 1.0 or self.presence_penalty != 0.0 or self.frequency_penalty != 0.0
+
+    @property
+    def adjusts(self) -> bool:
+        """Whether logits are adjusted at all."""
+        return self.penalizes or bool(self.logit_bias) or self.allowed is not None
 
 
-__all__ = ["SamplingParams"]
+def pack_allowed(allowed, vocab: int) -> Optional[np.ndarray]:
+    """A set of token ids as the mask that the kernel takes: int32 [ceil(vocab / 32)], bit t % 32 of word t // 32.  An array
+    of that type and shape is taken to be one already.  None if nothing is allowed."""
+    words = -(-vocab // 32)
+    if isinstance(allowed, np.ndarray) and allowed.dtype == np.int32 and allowed.shape == (words,):
+        tail = vocab % 32
+        last = int(allowed[-1]) & ((1 << tail) - 1 if tail else -1)
+        return np.ascontiguousarray(allowed) if last or allowed[:-1].any() else None
+    ids = np.fromiter((int(t) for t in allowed), dtype=np.int64)
+    if ids.size == 0:
+        return None
+    if ids.min() < 0 or ids.max() >= vocab:
+        raise ValueError(f"allowed tokens from {ids.min()} to {ids.max()} with a vocabulary of {vocab}")
+    bits = np.zeros(words * 32, dtype=np.uint8)
+    bits[ids] = 1
+    return np.packbits(bits, bitorder="little").view("<i4")
+
+
+__all__ = ["MAX_BIASES", "SamplingParams", "pack_allowed"]
