@@ -14,28 +14,27 @@ struct SharedLists {
 
 constexpr int TC_ROWS = 128;                     // query rows of a large family's unit
 constexpr int TC_SMEM_MOST = 112 * 1024;         // two blocks an SM
+constexpr long long TC_PRODUCTS = 1 << 18;
 
-// Whether a family of n tokens goes to the kernel for large ones: see attention_shared_tc.cu.
-__host__ __device__ inline bool tc_family(int n, int G, int shared) { return n * G > 32 && shared > 0; }
+// Whether a family of n tokens goes to the kernel for large ones: by its products, rows x keys.  Measured (us a call in a graph,
+// keys in no cache, 8 KV heads of 128, a hundred keys of its own a token; that kernel / units of 16 rows): 64 rows behind 1,024
+// keys 25 / 18, 4,096 28 / 29, 8,192 30 / 47; 128 rows behind 1,024 30 / 25, 4,096 34 / 49; 256 rows behind 256 33 / 28, 1,024
+// 37 / 37, 4,096 44 / 86, 8,192 53 / 150.
+__host__ __device__ inline bool tc_family(int n, int G, int shared) {
+    return n * G > 32 && (long long)n * G * shared >= TC_PRODUCTS;
+}
 // Units that the large families of M members in R groups can have: each has more than 32 rows.
 __host__ __device__ inline int tc_units(int M, int R, int G) {
     const int families = M * G / 33;
     return M * G / TC_ROWS + (families < R ? families : R);
 }
 
-// How T tiles are cut: `first` pieces of equal length (one a block) that hold the first T1 tiles, then `more` (possibly none)
-// shorter ones, which the blocks claim one after the other.
+// T tiles in `pieces` pieces of equal length.
 struct Cut {
-    int T, first, T1, more;
-    __device__ __forceinline__ int pieces() const { return first + more; }
-    __device__ __forceinline__ int begin(int c) const {
-        return c <= first ? (int)((long long)c * T1 / first) : T1 + (int)((long long)(c - first) * (T - T1) / more);
-    }
+    int T, pieces;
+    __device__ __forceinline__ int begin(int c) const { return (int)((long long)c * T / pieces); }
     // the piece that tile x lies in
-    __device__ __forceinline__ int of(int x) const {
-        return x < T1 ? (int)(((long long)(x + 1) * first + T1 - 1) / T1) - 1
-                      : first + (int)(((long long)(x - T1 + 1) * more + (T - T1) - 1) / (T - T1)) - 1;
-    }
+    __device__ __forceinline__ int of(int x) const { return (int)(((long long)(x + 1) * pieces + T - 1) / T) - 1; }
     // Where the partial results of an item with tiles [from, end) lie: its first piece (bit 31: that piece's second result, as
     // the end of another item is its first) and the end of its pieces.
     __device__ __forceinline__ int2 parts(int from, int end) const {

@@ -5,11 +5,14 @@
 // a family's shared keys 16 of its tokens x G rows at a time, so both kinds of work are the same walk.
 //
 // An item is one set of rows with the keys that all of them meet: first the families' units of 16 rows, then the tokens.
-// The 64-key tiles of all items are laid end to end (per KV head) and cut into equal chunks: one a block where there is
-// little to do, else up to four, of which the blocks claim one after the other (a block that starts late, behind the kernel for
-// large families, takes fewer).  The cut is made on the device, so a recorded graph follows the lists.  Every item leaves
-// partial results (max, sum, O): one if it lies in one chunk, one per chunk otherwise.  A second kernel joins a token's
-// own and its unit's partial results in key order: the same bits every time, whoever took a chunk.
+// The 64-key tiles of all items are laid end to end (per KV head) and dealt to the GPU's blocks in equal shares, as in
+// attention_balanced.cu; the cut is made on the device, so a recorded graph follows the lists.  Every item leaves partial
+// results (max, sum, O): one if it lies in one share, one per share otherwise.  A second kernel joins a token's own
+// and its unit's partial results in key order: no atomics, the same bits every time.
+//
+// (Chunks of tiles that blocks claim, beside one block an SM of the kernel for large families instead of behind two: 106 us for
+// 64 rows behind 6,144 keys with up to 2,048 of their own, 91 so.  What the claims add to the loop over tiles costs it a tenth,
+// and a block of either kernel is slower beside one of the other.)
 #include <math.h>
 
 #include "attention_mma.cuh"
@@ -19,13 +22,11 @@ namespace {
 
 constexpr int NW = 4;                    // warps of a block; a tile holds 16 keys for each
 constexpr int STAGES = 3;
-constexpr int AHEAD = 3;                 // tiles that page numbers are read ahead (their copies go out STAGES - 1 ahead)
-constexpr int CHUNK = AHEAD + 3;         // tiles of a claimed chunk at least
+constexpr int AHEAD = 7;                 // tiles that page numbers are read ahead (their copies go out STAGES - 1 ahead)
 constexpr int PAGE_SLOTS = 8;            // tiles whose page numbers are held: more than AHEAD, a power of two
 constexpr int TILE_PAGES = 4;            // pages of 16 keys and more
 constexpr int RQ = 16;                   // rows of an item: two column blocks
 constexpr int SMEM_MOST = 220 * 1024, TWO_AN_SM = 112 * 1024;      // dynamic shared memory of a block
-constexpr int MAX_KV_HEADS = 256;
 constexpr int MAX_MEMBERS = 512;         // (their lists live in shared memory)
 
 // Units of 16 rows that the families of M members can have.
@@ -33,8 +34,7 @@ __host__ __device__ inline int most_units(int M, int R, int G) { return M * G / 
 
 struct StreamArgs {
     float *whole_o, *whole_ml;           // [Hkv][items][16][D] and [Hkv][items][16][2]
-    float *piece_o, *piece_ml;           // [Hkv][4 W][2][16][D] and [Hkv][4 W][2][16][2]
-    int* counters;                       // [Hkv] chunks claimed, zero before and after
+    float *piece_o, *piece_ml;           // [Hkv][W][2][16][D] and [Hkv][W][2][16][2]
     int* items;                          // for the joining kernel: eight entries a member (see sb::TcPart), -2 first: not served
     const bf16 *q, *k_pool, *v_pool;
     const int *block_table, *token_rows, *positions, *members, *group_starts, *shared_lens;
@@ -64,16 +64,9 @@ __host__ __device__ inline int list_ints(int M, int R, int units) { return 4 * M
 struct Cursor {
     int i, begin, end, lo, hi, first;    // first: the tile index inside the row of flat tile 0
     const int* table;
+    // (item by item: the loop over tiles holds this code three times)
     __device__ __forceinline__ void seek(int x, const Lists& it, const StreamArgs& a) {
-        if (x >= it.pre[i + 1]) ++i;                         // the next one, or (after a jump, or behind empty items) a later one
-        if (x >= it.pre[i + 1]) {
-            int top = it.I - 1;
-            while (i < top) {
-                const int mid = (i + top) / 2;
-                if (x >= it.pre[mid + 1]) i = mid + 1;
-                else top = mid;
-            }
-        }
+        while (x >= it.pre[i + 1]) ++i;
         begin = it.pre[i];
         end = it.pre[i + 1];
         lo = it.lo(i);
@@ -83,15 +76,6 @@ struct Cursor {
     }
     __device__ __forceinline__ int tile_start(int x) const { return (first + x) * KT; }
 };
-
-// The cut for W blocks.  Few tiles: equal chunks, one a block.  More: a block's own chunk is three fifths of an equal share, and
-// the rest goes in chunks of five tiles and more to whoever is done.  (Equal shares alone: a block that starts 20 us late, behind
-// the kernel for large families, ends 20 us late.)
-__device__ __forceinline__ sb::Cut cut_of(int T, int W) {
-    if (T < 15 * W) return sb::Cut{T, max(1, min(W, T)), T, 0};
-    const int T1 = T / 5 * 3;
-    return sb::Cut{T, W, T1, min(3 * W, (T - T1) / CHUNK)};
-}
 
 // Running sum over `n` values in shared memory, v[0] = 0 .. v[n]: v[i + 1] holds the i-th value when it is called.
 __device__ __forceinline__ void running_sum(int* v, int n, int* scan) {
@@ -120,14 +104,14 @@ __device__ __forceinline__ void running_sum(int* v, int n, int* scan) {
     __syncthreads();
 }
 
-template <int D>
+// `large`: the large families' shared keys are the kernel's before this one.
+template <int D, bool large>
 __global__ void __launch_bounds__(32 * NW, 2) shared_stream_kernel(const StreamArgs a) {
     sb::pdl_launch_dependents();
     // Before pdl_wait(): the lists, positions, block table (host copies) and keys and values below a row's newest position
-    // (earlier steps).  Behind the kernel for large families, which lets this one in when its own wait has returned, queries
-    // and newest keys are complete too (and the partial results of an earlier call are read): this one then runs beside it
-    // and waits for it at its end, for the joining kernel's sake.
-    const bool large = a.tc.items != nullptr;
+    // (earlier steps).  Behind the kernel for large families, which lets this one in when its own wait has returned (if there is a
+    // large family), queries and newest keys are complete too, and the partial results of an earlier call are read: this
+    // one then waits for it only at its end, for the joining kernel's sake.
     constexpr int NTHR = 32 * NW;
     constexpr int STAGE = 2 * KT * D;                       // elements of a stage: keys, then values
     extern __shared__ __align__(128) uint8_t smem[];
@@ -149,18 +133,24 @@ __global__ void __launch_bounds__(32 * NW, 2) shared_stream_kernel(const StreamA
     it.unit_hi = it.unit_lo + units;
     it.pre = it.unit_hi + units;
     __shared__ float w_m[NW][16], w_l[NW][16];
-    __shared__ int s_scan[NW], s_item0, s_next;
+    __shared__ int s_scan[NW], s_large;
 
     const int bs_log2 = 31 - __clz(a.BS);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int kh = blockIdx.x % a.Hkv, slot = blockIdx.x / a.Hkv;
 
     // ---- the lists, then the items and their tiles
+    if constexpr (large) {
+        if (tid == 0) s_large = 0;
+        __syncthreads();
+    }
     for (int i = tid; i < a.R; i += NTHR) {
         const int s0 = a.group_starts[i], n = a.group_starts[i + 1] - s0;
         it.starts[i] = s0;
         const int shared = a.shared_lens[i];
-        it.uoff[i + 1] = shared > 0 && !(large && sb::tc_family(n, G, shared)) ? (n * G + RQ - 1) / RQ : 0;
+        const bool elsewhere = large && sb::tc_family(n, G, shared);
+        if (elsewhere) s_large = 1;
+        it.uoff[i + 1] = shared > 0 && !elsewhere ? (n * G + RQ - 1) / RQ : 0;
     }
     if (tid == 0) it.starts[a.R] = a.group_starts[a.R];
     for (int i = tid; i < a.M; i += NTHR) {
@@ -171,6 +161,7 @@ __global__ void __launch_bounds__(32 * NW, 2) shared_stream_kernel(const StreamA
     }
     __syncthreads();
     running_sum(it.uoff, a.R, s_scan);
+    const bool behind = large && s_large != 0;
     const int U = it.U = it.uoff[a.R], served = min(a.M, it.starts[a.R]), I = it.I = U + served;
     auto family_of = [&](const int* begin, int x) {         // the last one that begins at x or before
         int r = 0, top = a.R - 1;
@@ -202,10 +193,9 @@ __global__ void __launch_bounds__(32 * NW, 2) shared_stream_kernel(const StreamA
     __syncthreads();
     running_sum(it.pre, I, s_scan);
     const int T = it.pre[I];
-    const sb::Cut cut = cut_of(T, a.W);
-    const int C = cut.pieces();
+    const sb::Cut cut{T, max(1, min(a.W, T))};
     if (blockIdx.x == 0) {
-        if (!large) sb::pdl_wait();                         // the previous call's joining kernel may still read this
+        if (!behind) sb::pdl_wait();                        // the previous call's joining kernel may still read this
         int4* where = reinterpret_cast<int4*>(a.items);
         for (int i = tid; i < a.M; i += NTHR) {
             int4 w = make_int4(i < served ? -1 : -2, 0, 0, 0), v = make_int4(0, 0, 0, it.token[i]);
@@ -224,17 +214,13 @@ __global__ void __launch_bounds__(32 * NW, 2) shared_stream_kernel(const StreamA
             where[2 * i + 1] = v;
         }
     }
-    if (slot >= cut.first || T == 0) {
+    if (slot >= cut.pieces || T == 0) {
         sb::pdl_wait();
         return;
     }
-    int chunk = slot, x0 = cut.begin(slot), x1 = cut.begin(slot + 1);       // the chunk that is worked on
-    for (int i = tid; i < I; i += NTHR)
-        if (it.pre[i] <= x0 && x0 < it.pre[i + 1]) s_item0 = i;
-    __syncthreads();
-
+    const int x0 = cut.begin(slot), x1 = cut.begin(slot + 1);
     const int n_pages = max(1, KT >> bs_log2);              // logical pages a tile touches
-    // Bring the physical page of entry e of tile x, the block's at-th, to its slot (0 where the item does not reach: such keys are never
+    // Bring the physical page of entry e of tile x, the share's at-th, to its slot (0 where the item does not reach: such keys are never
     // read, see load_kv_tile).  Asynchronous: part of the commit group that is open.
     auto fetch_page = [&](const Cursor& c, int x, int at, int e) {
         const int logical = (c.tile_start(x) >> bs_log2) + e;
@@ -244,18 +230,6 @@ __global__ void __launch_bounds__(32 * NW, 2) shared_stream_kernel(const StreamA
                        "l"(c.table + (valid ? logical : 0)), "r"(valid ? 4 : 0)
                      : "memory");
     };
-    for (int i = tid; i < AHEAD * n_pages; i += NTHR) {
-        const int x = x0 + i / n_pages;
-        if (x < x1) {
-            Cursor c;
-            c.i = s_item0;
-            c.seek(x, it, a);
-            fetch_page(c, x, i / n_pages, i % n_pages);
-        }
-    }
-    cp_async_commit();
-    cp_async_wait<0>();
-    __syncthreads();
     // flat row f of the members' rows: token f / G of the members, head kh G + f % G
     auto load_query = [&](const Cursor& c, int stage) {
         constexpr int CH = D / 8;
@@ -270,14 +244,35 @@ __global__ void __launch_bounds__(32 * NW, 2) shared_stream_kernel(const StreamA
         }
     };
 
+    const WholeTileCopy<D, KT, NTHR> copy(ring, ring + KT * D, STAGE, a.k_pool, a.v_pool, bs_log2, a.Hkv, kh);
+    ColState<D, 2> st;
+    st.init();
+    uint32_t qf[D / 16][4];
+    int cpos[4], clo[4];                                    // the keys that this thread's columns see
+    Cursor c0;                                              // of the share's first tile
+    c0.i = 0;
+    for (int top = I - 1; c0.i < top;) {
+        const int mid = (c0.i + top) / 2;
+        if (x0 >= it.pre[mid + 1]) c0.i = mid + 1;
+        else top = mid;
+    }
+    c0.seek(x0, it, a);
+    for (int i = tid; i < AHEAD * n_pages; i += NTHR) {
+        const int x = x0 + i / n_pages;
+        if (x < x1) {
+            Cursor c = c0;
+            if (x >= c.end) c.seek(x, it, a);
+            fetch_page(c, x, i / n_pages, i % n_pages);
+        }
+    }
+    cp_async_commit();
+    cp_async_wait<0>();
+    __syncthreads();
     // ---- the first tiles: those of shared keys and those below their token's newest key before the wait, the others after it
-    Cursor cl;                                              // of the tile whose copies go out
-    cl.i = s_item0;
-    cl.seek(x0, it, a);
-    const Cursor c0 = cl;
+    Cursor cl = c0;                                         // of the tile whose copies go out
 #pragma unroll
     for (int late = 0; late < 2; ++late) {
-        if (late && !large) sb::pdl_wait();
+        if (late && !behind) sb::pdl_wait();
         cl = c0;
 #pragma unroll
         for (int s = 0; s < STAGES - 1; ++s) {
@@ -295,41 +290,17 @@ __global__ void __launch_bounds__(32 * NW, 2) shared_stream_kernel(const StreamA
 #pragma unroll
     for (int s = 1; s < STAGES - 1; ++s) cp_async_commit();
 
-    // Chunks beyond the blocks' first ones are claimed when AHEAD + 3 tiles of the chunk before are left: no earlier, so that a block
-    // that is slow or late claims less.
-    int claimed = C, next_chunk = C, nx0 = 0, nx1 = 0;
-    // the tile `k` after tile x of this block, or -1
-    auto ahead = [&](int x, int k) {
-        const int y = x + k;
-        return y < x1 ? y : y - x1 < nx1 - nx0 ? nx0 + y - x1 : -1;
-    };
-
-    const WholeTileCopy<D, KT, NTHR> copy(ring, ring + KT * D, STAGE, a.k_pool, a.v_pool, bs_log2, a.Hkv, kh);
-    ColState<D, 2> st;
-    st.init();
-    uint32_t qf[D / 16][4];
-    int cpos[4], clo[4];                                    // the keys that this thread's columns see
     Cursor cc = c0, ct = c0;                                // of the tile that is computed, and of the page read-ahead
-    int stage = STAGES - 1;                                 // of the block's at-th tile: at % STAGES
-    for (int x = x0, at = 0;; ++at) {
+    int stage = STAGES - 1;                                 // of tile x: (x - x0) % STAGES
+    for (int x = x0; x < x1; ++x) {
         stage = stage == STAGES - 1 ? 0 : stage + 1;
         cp_async_wait<STAGES - 2>();
         __syncthreads();                                    // tile x is there; everybody is done with the tile before
-        if (cut.more > 0) {
-            const int left = x1 - x;
-            if (left == AHEAD + 3 && tid == 0) claimed = cut.first + atomicAdd(a.counters + kh, 1);
-            if (left == AHEAD + 2 && tid == 0) s_next = claimed;
-            if (left == AHEAD + 1) {
-                next_chunk = s_next;
-                nx0 = next_chunk < C ? cut.begin(next_chunk) : 0;
-                nx1 = next_chunk < C ? cut.begin(next_chunk + 1) : 0;
-            }
-        }
-        const int xt = ahead(x, AHEAD), xl = ahead(x, STAGES - 1);
-        if (xl >= cl.end) cl.seek(xl, it, a);
-        if (xt >= 0) {
+        const int xt = x + AHEAD, xl = x + STAGES - 1;
+        if (xl < x1 && xl >= cl.end) cl.seek(xl, it, a);
+        if (xt < x1) {
             if (xt >= ct.end) ct.seek(xt, it, a);
-            if (tid < n_pages) fetch_page(ct, xt, at + AHEAD, tid);
+            if (tid < n_pages) fetch_page(ct, xt, xt - x0, tid);
         }
         if (x >= cc.end) cc.seek(x, it, a);
         const int nr = it.rows(cc.i);
@@ -348,17 +319,17 @@ __global__ void __launch_bounds__(32 * NW, 2) shared_stream_kernel(const StreamA
         }
         // the copies of tile xl: in doses between the phases of tile x, or (a tile at an item's edge) at once
         const int stage_l = stage == 0 ? STAGES - 1 : stage - 1;
-        const int* pg_l = pages + ((at + STAGES - 1) % PAGE_SLOTS) * TILE_PAGES;
+        const int* pg_l = pages + ((xl - x0) % PAGE_SLOTS) * TILE_PAGES;
         const int tl = cl.tile_start(xl);
         bool doses = false;
-        if (xl >= 0) {
+        if (xl < x1) {
             doses = tl >= cl.lo && tl + KT <= cl.hi;
             if (!doses) {
                 bf16* ks = ring + stage_l * STAGE;
                 load_kv_tile<D, KT, NTHR>(ks, ks + KT * D, a.k_pool, a.v_pool, pg_l, tl >> bs_log2, bs_log2, a.Hkv, kh, tl,
                                           cl.lo, cl.hi);
             }
-            if (xl == cl.begin || xl == nx0) load_query(cl, stage_l);
+            if (xl == cl.begin) load_query(cl, stage_l);
         }
         auto between = [&](int part) {
             if (doses) copy.dose(part, stage_l, pg_l - (tl >> bs_log2), tl);
@@ -373,13 +344,9 @@ __global__ void __launch_bounds__(32 * NW, 2) shared_stream_kernel(const StreamA
         if (nr <= 8) warp_tile_decode<D, 1>(st, qf, ks, ks + KT * D, warp * 16, ts, 0, 0, 0, 1.0f, false, between, seen);
         else warp_tile_decode<D, 2>(st, qf, ks, ks + KT * D, warp * 16, ts, 0, 0, 0, 1.0f, false, between, seen);
         cp_async_commit();
-        const bool chunk_ends = x + 1 == x1;
-        if (!chunk_ends && x + 1 != cc.end) {
-            ++x;
-            continue;
-        }
+        if (x + 1 != x1 && x + 1 != cc.end) continue;
 
-        // ---- the item, or this chunk of it, ends: merge the warps through the stage that was just read
+        // ---- the item, or this share of it, ends: merge the warps through the stage that was just read
         __syncthreads();
         float* wo = reinterpret_cast<float*>(ring + stage * STAGE);        // [NW][16][D]: exactly a stage
 #pragma unroll
@@ -404,8 +371,8 @@ __global__ void __launch_bounds__(32 * NW, 2) shared_stream_kernel(const StreamA
         }
         __syncthreads();
         st.init();
-        const bool whole = cc.begin >= x0 && cc.end <= x1;  // the item lies in this chunk
-        const size_t p = whole ? (size_t)kh * most + (cc.i < U ? cc.i : units + cc.i - U) : ((size_t)kh * 4 * a.W + chunk) * 2 + (cc.begin <= x0 ? 0 : 1);
+        const bool whole = cc.begin >= x0 && cc.end <= x1;  // the item lies in this share
+        const size_t p = whole ? (size_t)kh * most + (cc.i < U ? cc.i : units + cc.i - U) : ((size_t)kh * a.W + slot) * 2 + (cc.begin <= x0 ? 0 : 1);
         float* to_o = (whole ? a.whole_o : a.piece_o) + p * RQ * D;
         float* to_ml = (whole ? a.whole_ml : a.piece_ml) + p * RQ * 2;
         for (int idx = tid * 4; idx < nr * D; idx += NTHR * 4) {
@@ -426,18 +393,9 @@ __global__ void __launch_bounds__(32 * NW, 2) shared_stream_kernel(const StreamA
             *reinterpret_cast<float4*>(to_o + idx) = o;
             if (idx == row * D) *reinterpret_cast<float2*>(to_ml + 2 * row) = make_float2(m, l);
         }
-        ++x;
-        if (chunk_ends) {
-            if (next_chunk >= C) break;
-            chunk = next_chunk;
-            x = x0 = nx0;
-            x1 = nx1;
-            next_chunk = C;
-            nx0 = nx1 = 0;
-        }
     }
     cp_async_wait<0>();
-    if (large) sb::pdl_wait();
+    if (behind) sb::pdl_wait();
 }
 
 // grid (M, Hkv): the G rows of a token of one KV head from its unit's partial results, then its own, in key order.  The
@@ -446,14 +404,13 @@ __global__ void __launch_bounds__(32 * NW, 2) shared_stream_kernel(const StreamA
 constexpr int JOIN = 4;
 
 template <int D>
-__global__ void __launch_bounds__(128 * JOIN, 3)
+__global__ void __launch_bounds__(128 * JOIN, 2)
 shared_stream_join_kernel(bf16* __restrict__ out, const StreamArgs a, int groups) {
     sb::pdl_launch_dependents();
     __shared__ float4 s_o[JOIN - 1][128];
     __shared__ float2 s_ml[JOIN - 1][128];
     sb::pdl_wait();
     const int i = blockIdx.x, kh = blockIdx.y, G = a.Hq / a.Hkv;
-    if (i == 0 && threadIdx.x == 0) a.counters[kh] = 0;
     const int4 w = reinterpret_cast<const int4*>(a.items)[2 * i], v = reinterpret_cast<const int4*>(a.items)[2 * i + 1];
     if (w.x == -2) return;
     int4 tw = make_int4(-1, 0, 0, 0);
@@ -476,19 +433,22 @@ shared_stream_join_kernel(bf16* __restrict__ out, const StreamArgs a, int groups
             L = L * keep + f * ml.y;
             o.x = o.x * keep + f * x.x; o.y = o.y * keep + f * x.y; o.z = o.z * keep + f * x.z; o.w = o.w * keep + f * x.w;
         };
-        // the partial results of row `row` of an item of `rows` rows: `whole` is the place of the only one, `piece` that of the
-        // first of several
-        auto add = [&](int from, int end, size_t whole, size_t piece, int row, int rows, const float* whole_o, const float* whole_ml,
-                       const float* piece_o, const float* piece_ml) {
-            const int s0 = from & 0x7fffffff, n = end - s0;
-            if (n == 1) {
-                if (group == 0)
-                    take(__ldcg(reinterpret_cast<const float2*>(whole_ml + (whole * rows + row) * 2)),
-                         __ldcg(reinterpret_cast<const float4*>(whole_o + (whole * rows + row) * D + d)));
-                return;
-            }
-            constexpr int AT = 4;                           // partial results in flight a thread
-            for (int s = group; s < n; s += AT * groups) {
+        if (mine) {
+            // The partial results of this row's unit, then those of the token's own keys.  Of an item that lies in one share
+            // there is one in whole_*, of another one in piece_* for each share (its first share's second one, if bit 31 says so).
+            const int units = most_units(a.M, a.R, G), items = units + a.M;
+            const bool tc = tw.x >= 0;
+            const int rows = tc ? sb::TC_ROWS : RQ, place = tc ? tw.x : w.x, row = place + g, unit = row / rows;
+            const bool next = place >= 0 && unit > place / rows;
+            const int from = place < 0 ? 0 : tc ? (next ? tw.w : tw.y) : next ? w.w : w.y;
+            const int end = place < 0 ? 0 : tc ? (next ? tv : tw.z) : next ? v.x : w.z;
+            const int n_unit = end - (from & 0x7fffffff), n_own = v.z - (v.y & 0x7fffffff);
+            // result x of one of the two lists: its row's place among whole_* (n = 1) or piece_*
+            auto at = [&](int x, int n, int first, size_t whole, size_t pieces, int per, int r) {
+                return (n == 1 ? whole : pieces + 2 * ((first & 0x7fffffff) + x) + (x == 0 && first < 0 ? 1 : 0)) * per + r;
+            };
+            constexpr int AT = 6;                           // partial results in flight a thread
+            for (int s = group; s < n_unit + n_own; s += AT * groups) {
                 float2 ml[AT];
                 float4 x[AT];
 #pragma unroll
@@ -496,30 +456,27 @@ shared_stream_join_kernel(bf16* __restrict__ out, const StreamArgs a, int groups
                     const int y = s + u * groups;
                     ml[u] = make_float2(-INFINITY, 0.f);
                     x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (y < n) {
-                        const size_t p = (piece + 2 * (s0 + y) + (y == 0 && from < 0 ? 1 : 0)) * rows + row;
-                        ml[u] = __ldcg(reinterpret_cast<const float2*>(piece_ml + p * 2));
-                        x[u] = __ldcg(reinterpret_cast<const float4*>(piece_o + p * D + d));
+                    if (y >= n_unit + n_own) continue;
+                    const float *po, *pml;
+                    size_t p;
+                    if (y < n_unit && tc) {
+                        p = at(y, n_unit, from, (size_t)kh * sb::tc_units(a.M, a.R, G) + unit, (size_t)kh * 2 * a.tc.W, rows, row % rows);
+                        po = n_unit == 1 ? a.tc.whole_o : a.tc.piece_o;
+                        pml = n_unit == 1 ? a.tc.whole_ml : a.tc.piece_ml;
+                    } else {
+                        const bool own = y >= n_unit;
+                        const int n = own ? n_own : n_unit;
+                        p = at(own ? y - n_unit : y, n, own ? v.y : from, (size_t)kh * items + (own ? units + i : unit),
+                               (size_t)kh * 2 * a.W, RQ, own ? g : row % RQ);
+                        po = n == 1 ? a.whole_o : a.piece_o;
+                        pml = n == 1 ? a.whole_ml : a.piece_ml;
                     }
+                    ml[u] = __ldcg(reinterpret_cast<const float2*>(pml + p * 2));
+                    x[u] = __ldcg(reinterpret_cast<const float4*>(po + p * D + d));
                 }
 #pragma unroll
                 for (int u = 0; u < AT; ++u) take(ml[u], x[u]);
             }
-        };
-        if (mine) {
-            const int units = most_units(a.M, a.R, G);
-            const size_t first = (size_t)kh * (units + a.M), pieces = (size_t)kh * 8 * a.W;
-            if (tw.x >= 0) {
-                const int row = tw.x + g, unit = row / sb::TC_ROWS;
-                const bool next = unit > tw.x / sb::TC_ROWS;
-                add(next ? tw.w : tw.y, next ? tv : tw.z, (size_t)kh * sb::tc_units(a.M, a.R, G) + unit, (size_t)kh * 2 * a.tc.W,
-                    row % sb::TC_ROWS, sb::TC_ROWS, a.tc.whole_o, a.tc.whole_ml, a.tc.piece_o, a.tc.piece_ml);
-            } else if (w.x >= 0) {
-                const int row = w.x + g, unit = row / RQ;
-                const bool next = unit > w.x / RQ;
-                add(next ? w.w : w.y, next ? v.x : w.z, first + unit, pieces, row % RQ, RQ, a.whole_o, a.whole_ml, a.piece_o, a.piece_ml);
-            }
-            add(v.y, v.z, first + units + i, pieces, g, RQ, a.whole_o, a.whole_ml, a.piece_o, a.piece_ml);
         }
         if (group > 0) {
             s_ml[group - 1][t] = make_float2(M, L);
@@ -546,9 +503,9 @@ int blocks_of(int M, int R, int Hq, int Hkv, int D, int num_sms) {
     return w < 1 ? 1 : w;
 }
 
-template <int D>
+template <int D, bool large>
 int launch_stream(void* out, StreamArgs a, cudaStream_t stream) {
-    auto kernel = shared_stream_kernel<D>;
+    auto kernel = shared_stream_kernel<D, large>;
     const int G = a.Hq / a.Hkv, smem = stream_smem(a.M, a.R, G, D);
     static sb::OncePerDevice once_per_device;
     bool& configured = once_per_device.flag();
@@ -559,7 +516,7 @@ int launch_stream(void* out, StreamArgs a, cudaStream_t stream) {
     }
     sb::launch(kernel, dim3(a.W * a.Hkv), dim3(32 * NW), smem, stream, a);
     // (four groups where all blocks of four fit the GPU at once)
-    const int groups = a.M * a.Hkv <= 3 * a.num_sms ? JOIN : 2;
+    const int groups = a.M * a.Hkv <= 2 * a.num_sms ? JOIN : 2;
     sb::launch(shared_stream_join_kernel<D>, dim3(a.M, a.Hkv), dim3(groups * (G * D >= 512 ? 128 : G * D >= 256 ? 64 : 32)), 0, stream,
                (bf16*)out, a, groups);
     return 0;
@@ -570,7 +527,7 @@ int launch_stream(void* out, StreamArgs a, cudaStream_t stream) {
 namespace sb {
 
 bool shared_stream_supports(int M, int R, int Hq, int Hkv, int D, int page_size) {
-    if (Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq / Hkv > RQ || Hkv > MAX_KV_HEADS || M <= 0 || M > MAX_MEMBERS || R <= 0) return false;
+    if (Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq / Hkv > RQ || M <= 0 || M > MAX_MEMBERS || R <= 0) return false;
     if (!(D == 16 || D == 32 || D == 64 || D == 128)) return false;
     if (page_size < KT / TILE_PAGES || (page_size & (page_size - 1)) != 0) return false;
     return stream_smem(M, R, Hq / Hkv, D) <= SMEM_MOST;
@@ -580,10 +537,10 @@ bool shared_stream_supports(int M, int R, int Hq, int Hkv, int D, int page_size)
 void shared_stream_scratch(int M, int R, int Hq, int Hkv, int D, int page_size, int num_sms, long long* floats, long long* ints) {
     const int G = Hq / Hkv, items = most_units(M, R, G) + M;
     const long long blocks = 2ll * num_sms > Hkv ? 2ll * num_sms : Hkv;          // of all KV heads, two an SM
-    *floats = ((long long)Hkv * items + 8 * blocks) * RQ * (D + 2);
-    *ints = MAX_KV_HEADS + 8ll * M;
+    *floats = ((long long)Hkv * items + 2 * blocks) * RQ * (D + 2);
+    *ints = 8ll * M;
     if (shared_tc_supports(M, R, Hq, Hkv, D, page_size, 1)) {
-        *floats += ((long long)Hkv * tc_units(M, R, G) + 2 * (num_sms > Hkv ? num_sms : Hkv)) * TC_ROWS * (D + 2);
+        *floats += ((long long)Hkv * tc_units(M, R, G) + 2 * blocks) * TC_ROWS * (D + 2);
         *ints += 8ll * M;
     }
 }
@@ -597,9 +554,8 @@ int shared_stream(void* out, float* part, int* items, const void* q, const void*
     a.whole_o = part;
     a.whole_ml = a.whole_o + Hkv * most * RQ * D;
     a.piece_o = a.whole_ml + Hkv * most * RQ * 2;
-    a.piece_ml = a.piece_o + 8ll * Hkv * W * RQ * D;
-    a.counters = items;                  // the first entries, whatever the call: no other call's lists lie there
-    a.items = items + MAX_KV_HEADS;
+    a.piece_ml = a.piece_o + 2ll * Hkv * W * RQ * D;
+    a.items = items;
     a.q = (const bf16*)q; a.k_pool = (const bf16*)k_pool; a.v_pool = (const bf16*)v_pool;
     a.block_table = l.block_table; a.token_rows = l.token_rows; a.positions = l.positions;
     a.members = l.members; a.group_starts = l.group_starts; a.shared_lens = l.shared_lens;
@@ -608,20 +564,21 @@ int shared_stream(void* out, float* part, int* items, const void* q, const void*
     a.scale_log2 = scale * LOG2E;
     if (status != nullptr && shared_tc_supports(l.M, l.R, Hq, Hkv, D, page_size, num_pages)) {
         const long long units = tc_units(l.M, l.R, G);
-        a.tc.W = num_sms > Hkv ? num_sms / Hkv : 1;          // a block an SM: beside it stays room for one of the walk's
-        a.tc.whole_o = a.piece_ml + 8ll * Hkv * W * RQ * 2;
+        a.tc.W = 2 * num_sms > Hkv ? 2 * num_sms / Hkv : 1;
+        a.tc.whole_o = a.piece_ml + 2ll * Hkv * W * RQ * 2;
         a.tc.whole_ml = a.tc.whole_o + Hkv * units * TC_ROWS * D;
         a.tc.piece_o = a.tc.whole_ml + Hkv * units * TC_ROWS * 2;
         a.tc.piece_ml = a.tc.piece_o + 2ll * Hkv * a.tc.W * TC_ROWS * D;
         a.tc.items = a.items + 8ll * l.M;
         const int rc = shared_tc(a.tc, q, k_pool, v_pool, l, Hq, Hkv, D, page_size, num_pages, window, scale, status, stream);
         if (rc != 0) return rc;
+        return D == 64 ? launch_stream<64, true>(out, a, stream) : launch_stream<128, true>(out, a, stream);
     }
     switch (D) {
-        case 16: return launch_stream<16>(out, a, stream);
-        case 32: return launch_stream<32>(out, a, stream);
-        case 64: return launch_stream<64>(out, a, stream);
-        default: return launch_stream<128>(out, a, stream);
+        case 16: return launch_stream<16, false>(out, a, stream);
+        case 32: return launch_stream<32, false>(out, a, stream);
+        case 64: return launch_stream<64, false>(out, a, stream);
+        default: return launch_stream<128, false>(out, a, stream);
     }
 }
 

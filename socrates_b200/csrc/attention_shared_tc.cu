@@ -15,6 +15,10 @@
 // of one unit and the beginning of another (segments): the copies run on across them, and each segment leaves a
 // partial result (max, sum, O) for the joining kernel.
 //
+// 64 tokens (256 rows) behind 8,192 keys, 8 KV heads of 128: 1.2 us a tile and block, two blocks an SM, 1,024 tiles of 128 rows a
+// round in 8.5 us; about 10 us more until the first weights are there and 2 for the last results.  The whole call 53 us, 150 with units
+// of 16 rows alone, 298 where every row reads its own way (floor 5.4 us of bytes, 5.3 of products).
+//
 // Every wait on an mbarrier is bounded; a give-up sets *status, and the block still frees its TMEM.
 #include <cuda.h>
 #include <math.h>
@@ -237,33 +241,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constan
     tcgen05_fence_after();
     const uint32_t tmem = tmem_slot;
     const int T = U > 0 ? pre[U] : 0, W = max(1, min(a.part.W, T));
-    const sb::Cut cut{T, W, T, 0};
-    // The kernel behind this one goes on from what was complete before this one's wait returned (queries, pages), beside
-    // this one: it is let in only now.
-    sb::pdl_wait();
-    sb::pdl_launch_dependents();
-    if (blockIdx.x == 0) {                                  // for the joining kernel
-        int4* where = reinterpret_cast<int4*>(a.part.items);
-        for (int i = tid; i < M; i += THREADS) {
-            int r = 0, top = R - 1;
-            while (r < top) {
-                const int mid = (r + top + 1) / 2;
-                if (starts[mid] <= i) r = mid;
-                else top = mid - 1;
-            }
-            int4 w = make_int4(-1, 0, 0, 0);
-            int rest = 0;
-            if (uoff[r + 1] > uoff[r]) {
-                w.x = uoff[r] * ROWS + (i - starts[r]) * G;
-                const int u = w.x / ROWS;
-                const int2 first = cut.parts(pre[u], pre[u + 1]), second = cut.parts(pre[u + 1], pre[min(u + 2, U)]);
-                w.y = first.x; w.z = first.y; w.w = second.x;
-                rest = second.y;
-            }
-            where[2 * i] = w;
-            a.part.items[8 * i + 4] = rest;
-        }
-    }
+    const sb::Cut cut{T, W};
     const bool active = slot < W && T > 0;
     const int x0 = active ? cut.begin(slot) : 0, x1 = active ? cut.begin(slot + 1) : 0;
     auto segment_at = [&](int x, int from) {                // the segment that begins with flat tile x; units before `from` end earlier
@@ -287,6 +265,45 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constan
         atomicExch(&abort_flag, 1);
     };
 
+    // (a softmax thread's query row)
+    auto query_row = [&](const Segment& s) {
+        const int f = s.row0 + min(tid, s.nr - 1), i = f / G;
+        return reinterpret_cast<const uint4*>(a.q + ((size_t)token[i] * a.Hq + kh * G + f - i * G) * D);
+    };
+    Segment seg0{};
+    const uint4* src0 = nullptr;
+    if (active && warp < 4) {
+        seg0 = segment_at(x0, 0);
+        src0 = query_row(seg0);
+    }
+    // The kernel behind this one goes on from what was complete before this one's wait returned (queries, pages): it is let in
+    // only then, and its blocks start where blocks of this one end.  Without a large family it does its own waiting, for
+    // this kernel, which ends when its first block has waited: the other blocks make room at once.
+    if (U == 0) sb::pdl_launch_dependents();
+    if (U > 0 || blockIdx.x == 0) sb::pdl_wait();
+    if (U > 0) sb::pdl_launch_dependents();
+    if (blockIdx.x == 0) {                                  // for the joining kernel
+        int4* where = reinterpret_cast<int4*>(a.part.items);
+        for (int i = tid; i < M; i += THREADS) {
+            int r = 0, top = R - 1;
+            while (r < top) {
+                const int mid = (r + top + 1) / 2;
+                if (starts[mid] <= i) r = mid;
+                else top = mid - 1;
+            }
+            int4 w = make_int4(-1, 0, 0, 0);
+            int rest = 0;
+            if (uoff[r + 1] > uoff[r]) {
+                w.x = uoff[r] * ROWS + (i - starts[r]) * G;
+                const int u = w.x / ROWS;
+                const int2 first = cut.parts(pre[u], pre[u + 1]), second = cut.parts(pre[u + 1], pre[min(u + 2, U)]);
+                w.y = first.x; w.z = first.y; w.w = second.x;
+                rest = second.y;
+            }
+            where[2 * i] = w;
+            a.part.items[8 * i + 4] = rest;
+        }
+    }
     if (!active) {
     } else if (copier) {
         // Tile t's keys go to K buffer t&1 once QK(t-2) has read it, its values to V buffer t&1 once PV(t-2) has.  Each lane
@@ -379,7 +396,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constan
         bool ok = true;
         int i = 0, u = 0;
         while (ok && x0 + i < x1) {
-            const Segment s = segment_at(x0 + i, u);
+            const Segment s = i == 0 ? seg0 : segment_at(x0 + i, u);
             u = s.unit;
             // ---- Q: flat row row0 + r is head r % G of a member, into the swizzled panels, a row by D / 8 neighbouring threads.
             // The score products of the segment before have read theirs: their last scores were met here.
@@ -389,8 +406,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constan
                 constexpr int CH = D / 8;
                 uint4 v[CH];
                 const bool mine = tid < s.nr;
-                const int f = s.row0 + (mine ? tid : 0), i = f / G;
-                const uint4* src = reinterpret_cast<const uint4*>(a.q + ((size_t)token[i] * a.Hq + kh * G + f - i * G) * D);
+                const uint4* src = i == 0 ? src0 : query_row(s);
 #pragma unroll
                 for (int c = 0; c < CH; ++c) v[c] = mine ? __ldcg(src + c) : make_uint4(0, 0, 0, 0);
                 uint8_t* to = gen_base + tid * 128;
@@ -588,7 +604,7 @@ namespace sb {
 
 bool shared_tc_supports(int M, int R, int Hq, int Hkv, int D, int page_size, long long num_pages) {
     if (!(D == 64 || D == 128) || !(page_size == 16 || page_size == 32 || page_size == 64)) return false;
-    if (!tc_family(M, Hq / Hkv, 1)) return false;            // no family can be large
+    if (M * (Hq / Hkv) <= 32) return false;                 // no family can be large
     if (num_pages <= 0 || num_pages * Hkv * page_size >= (1ll << 31)) return false;
     return tc_smem<128>(M, R, Hq / Hkv) <= TC_SMEM_MOST;
 }

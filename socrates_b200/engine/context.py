@@ -123,7 +123,7 @@ class StepContext:
         self.host_batch = host_batch        # the host-side entries; None while a graph is recorded
         self.share_keys = share_keys        # a decode step whose rows differ much (see Model.prefers_shares)
         # (members, starts, lengths) of the requests of one token whose rows share keys (see ops.attention_shared), int32 on the
-        # device; None: not worth its launches, or nobody shares
+        # device, and whether one of the families is large; None: not worth its launches, or nobody shares
         self.families = families
         # keys of the longest request that brings one token (0: there is none, or the step is being recorded)
         self.longest_single = max((e.start + 1 for e in host_batch or () if len(e.tokens) == 1), default=0)

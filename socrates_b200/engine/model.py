@@ -120,6 +120,9 @@ class Model:
         optional `prefers_families`)."""
         return any(p.prefers_families(shared) for p in self._family_readers)
 
+    def has_large_family(self, shared) -> bool:
+        return any(p.has_large_family(shared) for p in self._family_readers)
+
     # ------------------------------------------------------------------ one step
     def _like_another(self, ctx: StepContext, stream: ResidualStream, view: CacheView, i: int,
                       recordings: Dict[tuple, tuple]) -> bool:

@@ -277,8 +277,8 @@ class ModelRunner:
         return N, M, R, all_decode, max_ctx
 
     def _context(self, N: int, M: int, R: int, all_decode: bool, max_ctx: int, host_batch,
-                 share_keys: bool = False, members: int = 0) -> StepContext:
-        """`members`: requests of one token in the families that were filled in (0: none)."""
+                 share_keys: bool = False, members: int = 0, large: bool = False) -> StepContext:
+        """`members`: requests of one token in the families that were filled in (0: none), one of which is `large`."""
         L, m = self.layout, self.dev_meta
         return StepContext(
             self.dtype, self.device, self.buffers, N, R,
@@ -289,7 +289,7 @@ class ModelRunner:
             all_decode=all_decode, max_context=max_ctx, host_batch=host_batch, num_sms=self.num_sms,
             status=self.status, token_feedback=self.sampled, share_keys=share_keys,
             families=(m[L.members:L.members + members], m[L.starts:L.starts + members + 1],
-                      m[L.shared:L.shared + members]) if members else None)
+                      m[L.shared:L.shared + members], large) if members else None)
 
     def begin_read(self, count: int) -> Tuple[int, int]:
         """Start the copy of the `count` tokens the last step sampled (and of the kernels'
@@ -388,10 +388,10 @@ class ModelRunner:
         return logits, tokens
 
     def _families(self, entries: Sequence[StepEntry]):
-        """(members, starts, shared lengths) of the entries of one token whose rows share keys, if reading those keys once
-        pays, else None.  Members are tokens of the step."""
+        """((members, starts, shared lengths) of the entries of one token whose rows share keys, whether a family is large), if
+        reading those keys once pays, else (None, False).  Members are tokens of the step."""
         if self.dtype != torch.bfloat16 or not any(self.cache.shared_len):
-            return None
+            return None, False
         tokens, rows, n = [], [], 0
         for e in entries:
             if len(e.tokens) == 1:
@@ -399,9 +399,10 @@ class ModelRunner:
                 rows.append(e.row)
             n += len(e.tokens)
         members, starts, shared = self.cache.families(rows)
-        if not self.model.prefers_families([(b - a, k) for a, b, k in zip(starts, starts[1:], shared)]):
-            return None
-        return [tokens[i] for i in members], starts, shared
+        sizes = [(b - a, k) for a, b, k in zip(starts, starts[1:], shared)]
+        if not self.model.prefers_families(sizes):
+            return None, False
+        return ([tokens[i] for i in members], starts, shared), self.model.has_large_family(sizes)
 
     def prepare(self, entries: Sequence[StepEntry],
                 sampling: Optional[Sequence[SamplingArgs]] = None) -> StepContext:
@@ -421,7 +422,7 @@ class ModelRunner:
         starts one past its row's committed length (and may name its token as -1 - j, the j-th
         token the step before sampled)."""
         self.cache.flush()
-        families = self._families(entries)
+        families, large = self._families(entries)
         N, M, R, all_decode, max_ctx = self._fill(entries, sampling, ahead, families)
         members = len(families[0]) if families is not None else 0
         sample = sampling is not None
@@ -437,9 +438,9 @@ class ModelRunner:
         self.steps_run += 1
         if self.use_graphs and all_decode and M == N:
             key = (N, sample, share)
-            key += tuple(name for name, on in (("families", members), ("tokens", self.cache.tokens is not None), ("adjust", adjust)) if on)
+            key += tuple(name for name, on in (("families", members), ("large", large), ("tokens", self.cache.tokens is not None), ("adjust", adjust)) if on)
             if key not in self._graphs and key in self._eager_decode_done:
-                ctx = self._context(N, M, R, True, self.cache.max_len, None, share, members)
+                ctx = self._context(N, M, R, True, self.cache.max_len, None, share, members, large)
                 graph = torch.cuda.CUDAGraph()
                 before = Counters.launches
                 with torch.cuda.graph(graph):
@@ -454,7 +455,7 @@ class ModelRunner:
                 return StepResult(logits, tokens, N)
             self._eager_decode_done.add(key)
             max_ctx = self.cache.max_len     # the same launch shapes the graph will record
-        ctx = self._context(N, M, R, all_decode, max_ctx, entries, share, members)
+        ctx = self._context(N, M, R, all_decode, max_ctx, entries, share, members, large)
         before = Counters.launches
         logits, tokens = self._run(ctx, M, sample, adjust)
         self.kernel_launches += Counters.launches - before

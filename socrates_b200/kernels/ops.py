@@ -371,11 +371,17 @@ def copy_pages(k_pools: torch.Tensor, v_pools: torch.Tensor, src: Sequence[int],
                                  value_page, _stream()), "copy_pages", kernels=lib.sb_copy_pages_kernels(n))
 
 
+def attention_shared_large(tokens: int, group: int, shared: int) -> bool:
+    """Whether a family of so many tokens of `group` query heads a KV head that shares so many keys goes through the kernel for
+    large families, if `attention_shared` is given a `status`."""
+    return bool(library().sb_attention_shared_large(tokens, group, shared))
+
+
 @functools.lru_cache(maxsize=None)
 def attention_shared_scratch_size(members: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int,
                                   dtype: torch.dtype) -> Tuple[int, int]:
     """(float32, int32) entries of scratch that `attention_shared` needs for up to so many members, in at most as many
-    groups; the int32 ones are zero before the first call."""
+    groups."""
     floats, ints = ctypes.c_longlong(), ctypes.c_longlong()
     lib = library()
     check(lib, lib.sb_attention_shared_scratch(members, num_heads, num_kv_heads, head_dim, page_size, _code(dtype),
@@ -396,9 +402,13 @@ def attention_shared(out: torch.Tensor, q: torch.Tensor, k_pool: torch.Tensor, v
     token's own position are not seen).  A token that shares nothing is a group of its own with length 0.  Tokens in no
     group are left alone in `out`.  group_starts int32 [groups + 1] starts at 0; empty groups may stand anywhere.
 
-    Scratch: `part` float32 and `lists` int32 of attention_shared_scratch_size() entries, allocated here if None; `lists` is
-    zero before its first use (the kernels leave it ready for the next call, of whatever shape).
-    `status`: int32 word for the bounded waits of the tensor-core kernel, which is not used without it."""
+    Scratch: `part` float32 and `lists` int32 of attention_shared_scratch_size() entries, allocated here if None.
+    `status`: int32 word for the bounded waits of the kernel for large families (attention_shared_large), which is not
+    launched without it; a call whose families are all small is 5 us faster so.
+
+    Read before the kernels wait for the one that precedes them on the stream, so these must be older than that one (a host
+    copy, an earlier step): the lists, rows, positions, the block table, and keys and values below each position.  A shared
+    value that only some tokens of a family see (through a window) must be finite: with bfloat16 it meets the others with weight 0."""
     N = q.shape[0]
     if k_pool.dim() != 4:
         raise KernelError(f"k_pool must be [pages, heads, slots, dim], got {tuple(k_pool.shape)}")
@@ -417,7 +427,7 @@ def attention_shared(out: torch.Tensor, q: torch.Tensor, k_pool: torch.Tensor, v
     if part is None or lists is None:
         floats, ints = attention_shared_scratch_size(M, Hq, Hkv, D, BS, q.dtype)
         part = torch.empty(floats, dtype=torch.float32, device=q.device) if part is None else part
-        lists = torch.zeros(ints, dtype=torch.int32, device=q.device) if lists is None else lists
+        lists = torch.empty(ints, dtype=torch.int32, device=q.device) if lists is None else lists
     _check(here, ((part, "part", torch.float32, None), (lists, "lists", i32, None)))
     if status is not None:
         _check(here, ((status, "status", i32, None),))

@@ -68,8 +68,14 @@ def decode_partitions(ctx, num_kv_heads: int, blocks_per_sm: int, keys_per_part:
 SINGLES_APART_FROM = 1024
 
 
-# From so many bytes of keys and values that need not be read again on, shared keys are read once.
-SHARED_PAYS_FROM = 48 << 20
+# From so many bytes of keys and values that need not be read again, for each query head of a KV head, on shared keys are read
+# once.  Measured (us a call in a graph, keys in no cache, 8 KV heads of 128, a hundred keys of its own a row; the faster of the
+# other decode kernels / shared; in brackets the MB saved), 32 query heads: 2 rows behind 8,192 keys (34) 16 / 21, 4 behind
+# 4,096 (50) 15 / 17, 4 behind 8,192 (101) 23 / 22, 8 behind 1,024 (29) 11 / 14, 8 behind 4,096 (117) 25 / 20, 16 behind 1,024 (63)
+# 16 / 18, 32 behind 1,024 (130) 24 / 25, 32 behind 4,096 (520) 77 / 34, 64 behind 256 (66) 21 / 28, 64 behind 1,024 (264) 48 / 37, 64
+# behind 8,192 (2,114) 298 / 53; 64 query heads: 4 behind 8,192 (101) 24 / 32, 8 behind 4,096 (117) 26 / 32, 8 behind 8,192 (235)
+# 44 / 37, 32 behind 1,024 (130) 25 / 34, 64 behind 1,024 (264) 49 / 44.
+SHARED_PAYS_FROM = 24_000_000
 
 
 def balanced_attention(ctx, out, q, k_pool, v_pool, table, num_heads: int, scale: float, window: int) -> None:
@@ -87,12 +93,12 @@ def balanced_attention(ctx, out, q, k_pool, v_pool, table, num_heads: int, scale
 def shared_attention(ctx, out, q, k_pool, v_pool, table, num_heads: int, scale: float, window: int) -> None:
     """The step's requests of one token through the kernels that read the keys of a family once, with scratch of the step."""
     Hkv, page_size, D = k_pool.shape[1], k_pool.shape[2], k_pool.shape[3]
-    members, starts, lengths = ctx.families
+    members, starts, lengths, large = ctx.families
     floats, ints = ops.attention_shared_scratch_size(members.numel(), num_heads, Hkv, D, page_size, q.dtype)
     take = ctx.buffers.take_flat
     ops.attention_shared(out, q, k_pool, v_pool, table, ctx.token_rows, ctx.positions, members, starts, lengths, num_heads, scale,
                          window, take("attn_shared_part", floats, torch.float32),
-                         take("attn_shared_lists", ints, torch.int32, zeroed=True), ctx.status)
+                         take("attn_shared_lists", ints, torch.int32), ctx.status if large else None)
 
 
 def paged_attention(ctx, out, q, k_pool, v_pool, table, num_heads: int, scale: float, window: int,
@@ -266,7 +272,11 @@ class GQAAttention(Part):
         if self.window or paged_partition() is not None:
             return False
         saved = sum((n - 1) * keys for n, keys in shared)
-        return saved * self.Hkv * self.D * 4 >= SHARED_PAYS_FROM
+        return saved * self.Hkv * self.D * 4 >= SHARED_PAYS_FROM * (self.Hq // self.Hkv)
+
+    def has_large_family(self, shared: Sequence[Tuple[int, int]]) -> bool:
+        """Whether one of these families is for the kernel for large ones."""
+        return any(ops.attention_shared_large(n, self.Hq // self.Hkv, keys) for n, keys in shared)
 
     def forward(self, ctx, x: torch.Tensor, cache) -> Branch:
         N = x.shape[0]

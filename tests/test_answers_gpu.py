@@ -67,8 +67,8 @@ class Rows:
     def __init__(self, rows, length, shape=WIDE, dtype=torch.bfloat16, graphs=True, more=3):
         config = config_from_dict(shape)
         _, model = build_random_model(config, 7, dtype, torch.device("cuda:0"))
-        self.cache = CacheManager(model.cache_needs(), rows + 2, 2048, 16, 400, dtype, "cuda:0")
-        self.runner = ModelRunner(model, self.cache, dtype, "cuda:0", max_tokens=1024, max_seqs=rows + 2, use_graphs=graphs)
+        self.cache = CacheManager(model.cache_needs(), rows + 2, 2048, 16, 500, dtype, "cuda:0")
+        self.runner = ModelRunner(model, self.cache, dtype, "cuda:0", max_tokens=1600, max_seqs=rows + 2, use_graphs=graphs)
         self.vocab = config.plan().vocab_size
         self.ids = {0: prompt(length, 3, self.vocab)}
         self.cache.assign(0)
@@ -94,7 +94,7 @@ class Rows:
         return logits
 
 
-@pytest.mark.parametrize("rows,length", [(2, 100), (5, 33), (14, 500), (3, 17)])
+@pytest.mark.parametrize("rows,length", [(2, 100), (5, 33), (14, 500), (3, 17), (48, 1500)])
 def test_a_step_with_families_gives_the_step_without(always_shared, monkeypatch, rows, length):
     both = []
     for on in (True, False):
@@ -107,6 +107,7 @@ def test_a_step_with_families_gives_the_step_without(always_shared, monkeypatch,
         out.append(r.feed({0: [8], rows: [3], rows - 1: [4]}))
         if on:
             assert any("families" in key for key in r.runner._graphs)
+            assert any("large" in key for key in r.runner._graphs) == (rows == 48)
         both.append(out)
     for a, b in zip(*both):
         # bfloat16 activations: a few roundings of 2^-9 of values that add up over four layers, as far as two correct kernels differ

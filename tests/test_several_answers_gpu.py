@@ -233,15 +233,27 @@ def test_attention_shared_of_more_members_than_the_lists_in_shared_memory_hold()
 
 
 def test_attention_shared_large_families_with_windows():
-    case = Case([(300, [1, 5, 50, 200] * 5), (160, [7] * 17 + [90])], 32, 8, 128, torch.bfloat16, seed=2)
-    for window in (3, 150, 290):
+    case = Case([(3300, [1, 5, 50, 200] * 5), (160, [7] * 7 + [90])], 32, 8, 128, torch.bfloat16, seed=2)
+    for window in (3, 150, 2900):
         check(case, case.run(window), case.want(window))
+
+
+@pytest.mark.parametrize("heads,shared", [((32, 8, 128), 4160), ((16, 8, 64), 6000), ((24, 2, 64), 1001)], ids=str)
+@pytest.mark.parametrize("own", [1, 60, 100, 200, 300, 420, 900])
+def test_attention_shared_beside_large_families(heads, shared, own):
+    """A family large enough for the kernel of its own, beside own keys of all lengths: few tiles and many, chunks that are
+    claimed one after the other and in advance; a small family and a lone token besides."""
+    n = -(-(1 << 18) // (shared * (heads[0] // heads[1]))) + 1
+    case = Case([(shared, [max(1, own - 7 * (i % 5)) for i in range(n)]), (64, [own, 3]), (0, [own])], *heads, torch.bfloat16, seed=own)
+    first = case.run()
+    check(case, first, case.want())
+    assert torch.equal(case.run(), first)
 
 
 @pytest.mark.parametrize("status", [True, False])
 def test_attention_shared_twice_is_the_same_bits(status):
     """Nothing is added in the order in which blocks come; with and without the kernel for large families."""
-    case = Case([(1500, [1, 70, 9] * 8), (64, [40, 3])], 32, 8, 128, torch.bfloat16, seed=9)
+    case = Case([(3500, [1, 70, 9] * 8), (64, [40, 3])], 32, 8, 128, torch.bfloat16, seed=9)
     first = case.run(status=status).clone()
     for _ in range(20):
         assert torch.equal(case.run(status=status), first)
