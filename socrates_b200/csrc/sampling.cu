@@ -176,7 +176,7 @@ constexpr int SLICE = 8192;          // logits of a block at most, held in share
 // most l can exceed it only where N - 1/2 <= 2^23 e^(l / T - F), a bound on the hash that a thread takes once, with its
 // largest logit.  The others are not looked at.
 // 64 rows of 151,936 logits, half of them drawn, tokens of up to 4,096 and 40 biases a row: 60 us a logit at a time with tables for
-// counts and biases, 42 with 16 logits a thread in registers, 31 so (22 if none is drawn, 14 if nothing is adjusted either).
+// counts and biases, 42 with 16 logits a thread in registers, 29 so (22 if none is drawn, 14 if nothing is adjusted either).
 __global__ void __launch_bounds__(512, 3)
 sample_adjusted_kernel(int* __restrict__ out, const float* __restrict__ logits, const float* __restrict__ temperature,
                        const uint32_t* __restrict__ seeds, const uint32_t* __restrict__ counters, int V, int per,
@@ -397,9 +397,13 @@ sample_adjusted_kernel(int* __restrict__ out, const float* __restrict__ logits, 
         // The bound on N and from it the one on the hash.  The exponent is enlarged by 2e-3 and 4e-6 of its terms, far more than the
         // roundings on both sides; whatever is not finite looks at everything.
         constexpr float LOG2E = 1.4426950408889634f;
-        const float l = best * inv_t, exponent = (l - least) * LOG2E + 2e-3f + 4e-6f * (fabsf(l) + fabsf(least));
-        const float bound = exponent < 0.f ? exp2f(23.0f + exponent) + 1.0f : 8388608.0f;
-        const uint32_t hash = (8388608u - (uint32_t)fminf(bound, 8388608.0f)) << 9;
+        auto bound = [&](float x) {
+            const float l = x * inv_t, exponent = (l - least) * LOG2E + 2e-3f + 4e-6f * (fabsf(l) + fabsf(least));
+            float e;
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(23.0f + exponent));
+            return exponent < 0.f ? e + 1.0f : 8388608.0f;
+        };
+        const uint32_t hash = (8388608u - (uint32_t)fminf(bound(best), 8388608.0f)) << 9;
         uint32_t look = 0;
         if (best_k >= 0) {                                  // else nothing of this thread's can win
 #pragma unroll
@@ -411,8 +415,11 @@ sample_adjusted_kernel(int* __restrict__ out, const float* __restrict__ logits, 
         while (look != 0) {                                 // in the order of the places
             const int k = __ffs(look) - 1;
             look &= look - 1;
-            const float4 x = four(k >> 2);
-            const float y = score((k & 3) == 0 ? x.x : (k & 3) == 1 ? x.y : (k & 3) == 2 ? x.z : x.w, k);
+            const float4 four_of = four(k >> 2);
+            const float x = (k & 3) == 0 ? four_of.x : (k & 3) == 1 ? four_of.y : (k & 3) == 2 ? four_of.z : four_of.w;
+            // the bound of this logit itself, which few pass: two logarithms are paid by the whole warp
+            if ((float)(8388608u - (mix32(((uint32_t)place(k) + 0x165667B1u) ^ key) >> 9)) > bound(x)) continue;
+            const float y = score(x, k);
             if (y > best) { best = y; best_k = k; }
         }
         __syncthreads();                                    // s_val is written again below
