@@ -69,13 +69,13 @@ SINGLES_APART_FROM = 1024
 
 
 # From so many bytes of keys and values that need not be read again, for each query head of a KV head, on shared keys are read
-# once.  Measured (us a call in a graph, keys in no cache, 8 KV heads of 128, a hundred keys of its own a row; the faster of the
-# other decode kernels / shared; in brackets the MB saved), 32 query heads: 2 rows behind 8,192 keys (34) 16 / 21, 4 behind
-# 4,096 (50) 15 / 17, 4 behind 8,192 (101) 23 / 22, 8 behind 1,024 (29) 11 / 14, 8 behind 4,096 (117) 25 / 20, 16 behind 1,024 (63)
-# 16 / 18, 32 behind 1,024 (130) 24 / 25, 32 behind 4,096 (520) 77 / 34, 64 behind 256 (66) 21 / 28, 64 behind 1,024 (264) 48 / 37, 64
-# behind 8,192 (2,114) 298 / 53; 64 query heads: 4 behind 8,192 (101) 24 / 32, 8 behind 4,096 (117) 26 / 32, 8 behind 8,192 (235)
-# 44 / 37, 32 behind 1,024 (130) 25 / 34, 64 behind 1,024 (264) 49 / 44.
-SHARED_PAYS_FROM = 24_000_000
+# once.  Measured in decode steps of the 4B shape (36 layers, 4 query heads a KV head, 100 to 160 tokens of its own a row; ms a step
+# without / with; in brackets the MB saved a layer): 8 rows behind 4,096 keys (117) 2.85 / 2.86, 16 behind 2,048 (126) 2.83 / 2.85, 32
+# behind 1,024 (130) 2.96 / 3.25, 24 behind 2,048 (193) 3.60 / 3.20, 8 behind 8,000 (229) 3.42 / 3.05, 64 behind 1,024 (264) 4.45 / 4.07,
+# 32 behind 4,096 (520) 5.44 / 3.74, 64 behind 8,000 (2,064) 14.22 / 4.94.  By the heads, because their rows are what the shared keys
+# are read for: launches of 64 query heads on 8 KV heads (us, the faster of the other kernels / this) 4 rows behind 8,192 (101)
+# 24 / 32, 8 behind 4,096 (117) 26 / 32, 8 behind 8,192 (235) 44 / 37, 64 behind 1,024 (264) 49 / 44.
+SHARED_PAYS_FROM = 36_000_000
 
 
 def balanced_attention(ctx, out, q, k_pool, v_pool, table, num_heads: int, scale: float, window: int) -> None:
