@@ -71,15 +71,38 @@ shared_rows_kernel(float* __restrict__ part_o, float* __restrict__ part_ml, cons
         hi = pos + 1;
         if (tid < RT) { r_mem[tid] = i; r_tok[tid] = n; r_head[tid] = kh * G + g0 + tid; r_pos[tid] = tid < n_rows ? pos : -1; }
     } else {
-        int r = 0, start = 0, rows = 0;
-        for (; r < a.R; ++r) {
-            start = a.group_starts[r];
-            rows = (a.group_starts[r + 1] - start) * G;
-            const int units = (rows + RT - 1) / RT;
-            if (u < units) break;
-            u -= units;
+        // the family that unit u belongs to: its thread finds it, THREADS families at a time
+        __shared__ int s_warp[THREADS / 32], s_found[3];
+        const int lane = tid & 31;
+        bool found = false;
+        for (int base = 0; base < a.R && !found; base += THREADS) {
+            const int r = base + tid, start = r < a.R ? a.group_starts[r] : 0;
+            const int rows = r < a.R ? (a.group_starts[r + 1] - start) * G : 0, units = (rows + RT - 1) / RT;
+            int to = units;                                  // units up to this family's end, of this round's
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, to, o);
+                if (lane >= o) to += up;
+            }
+            if (lane == 31) s_warp[tid >> 5] = to;
+            __syncthreads();
+            int total = 0;
+            for (int w = 0; w < THREADS / 32; ++w) {
+                if (w < tid >> 5) to += s_warp[w];
+                total += s_warp[w];
+            }
+            if (u < to && u >= to - units) {
+                s_found[0] = r;
+                s_found[1] = rows;
+                s_found[2] = u - (to - units);
+            }
+            found = u < total;
+            __syncthreads();
+            if (!found) u -= total;
         }
-        if (r == a.R) return;
+        if (!found) return;
+        const int r = s_found[0], rows = s_found[1], start = a.group_starts[r];
+        u = s_found[2];
         n_rows = min(RT, rows - u * RT);
         hi = a.shared_lens[r];
         if (tid < RT) {

@@ -539,7 +539,7 @@ void shared_stream_scratch(int M, int R, int Hq, int Hkv, int D, int page_size, 
     const long long blocks = 2ll * num_sms > Hkv ? 2ll * num_sms : Hkv;          // of all KV heads, two an SM
     *floats = ((long long)Hkv * items + 2 * blocks) * RQ * (D + 2);
     *ints = 8ll * M;
-    if (shared_tc_supports(M, R, Hq, Hkv, D, page_size, 1)) {
+    if (shared_tc_supports(M, 1, Hq, Hkv, D, page_size, 1)) {        // (lists of fewer families may fit where these do not)
         *floats += ((long long)Hkv * tc_units(M, R, G) + 2 * blocks) * TC_ROWS * (D + 2);
         *ints += 8ll * M;
     }

@@ -21,7 +21,7 @@ template <typename V, int N>
 __global__ void __launch_bounds__(THREADS)
 copy_pages_kernel(V* k, V* v, const __grid_constant__ Pairs<N> pairs, int n, long long k_run, long long v_run, int k_page,
                   int v_page, int pieces) {
-    // No launch_dependents: kernels that read pages before their own wait must find the copies done.
+    // No launch_dependents, and a fence at the end: kernels that read pages before their own wait must find the copies done.
     sb::pdl_wait();
     long long b = blockIdx.x;
     const int piece = (int)(b % pieces);
@@ -42,6 +42,7 @@ copy_pages_kernel(V* k, V* v, const __grid_constant__ Pairs<N> pairs, int n, lon
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u)
         if (at + u * THREADS < page) to[at + u * THREADS] = x[u];
+    __threadfence();
 }
 
 template <typename V, int N>

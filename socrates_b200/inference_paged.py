@@ -79,6 +79,8 @@ def main(argv=None) -> int:
     ap.add_argument("--prompt-len", type=int, default=32, help="length of the random prompts")
     args = ap.parse_args(argv)
 
+    if args.answers < 1:
+        ap.error("--answers must be at least 1")
     if os.environ.get("ENGINE", "paged") != "paged":
         print(f"ENGINE={os.environ['ENGINE']!r}: only the paged engine exists here", file=sys.stderr)
         return 2
