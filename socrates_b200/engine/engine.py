@@ -118,7 +118,7 @@ class Engine:
     def warmup(self) -> None:
         """Record one decode graph per batch width now instead of at the first step of each
         width (the reference warms all its widths in its constructor,
-        model/inference_paged.py:110-130)."""
+        model/inference_paged.py:110-130).  Steps that read shared keys once or adjust logits are recorded when they are met."""
         t0 = time.perf_counter()
         n = self.runner.warmup(self.max_batch)
         if n:
@@ -158,27 +158,25 @@ class Engine:
         allowed = sampling.get("allowed")
         if allowed is not None and not callable(allowed):
             sampling["allowed"] = allowed = list(allowed)    # an iterator is walked more than once
+        if sampling.get("logit_bias") is not None:
+            sampling["logit_bias"] = dict(sampling["logit_bias"])       # what the caller does to theirs later does not matter
         params = [SamplingParams(float(temperature), int(seed) + i, **sampling) for i in range(n)]
         params[0].validate(vocab)
-        if params[0].adjusts:
-            if vocab > MOST_ADJUSTED:
-                raise ValueError(f"logits of {vocab} tokens cannot be adjusted (at most {MOST_ADJUSTED})")
-            if params[0].penalizes:
-                self.cache.keep_tokens()    # from the prompt's first token on
+        if params[0].adjusts and vocab > MOST_ADJUSTED:
+            raise ValueError(f"logits of {vocab} tokens cannot be adjusted (at most {MOST_ADJUSTED})")
         if len(self.scheduler.pending) + n > self.scheduler.max_queue:
             raise QueueFull(f"{len(self.scheduler.pending)} requests already waiting, {n} more")
         mask = pack_allowed(allowed, vocab) if allowed is not None and not callable(allowed) else None
-        reqs = []
+        reqs: List[Request] = []
         for p in params:
             req = Request(ids=ids, max_new_tokens=max_new_tokens or self.max_new_tokens, sampling=p, prompt=text)
             req.mask = mask
+            if n > 1:
+                req.siblings = reqs
             if stream:
                 import queue
                 req.stream = queue.Queue()
             reqs.append(self.scheduler.submit(req))
-        if n > 1:
-            for req in reqs:
-                req.siblings = reqs
         return reqs
 
     # ------------------------------------------------------------------ stepping
@@ -190,6 +188,8 @@ class Engine:
         args = [SamplingArgs(t, s, c) for (t, s, c) in self.scheduler.sampling_args(plan)]
         for a, e in zip(args, (e for e in plan.entries if e.samples)):
             a.adjust = self._adjust(e.request, e.row, e.start + e.count)
+        if self.cache.tokens is None and any(e.request.sampling.penalizes for e in plan.entries):
+            self.cache.keep_tokens()        # before the first token of their prompts is computed
         result = self.runner.step(entries, args)
         return self.runner.begin_read(len(args)) if result.tokens is not None else None
 

@@ -220,7 +220,7 @@ def silu_mul(out: torch.Tensor, gate_up: torch.Tensor, interleaved: bool = False
 
 def sample_scratch_size(M: int, V: int) -> int:
     """int32 entries of scratch that `sample` and `sample_adjusted` need for M rows of V logits (a place each: calls of both
-    may share it)."""
+    may share it, as long as V is one)."""
     lib = library()
     return M * (2 * lib.sb_sample_slices(int(V)) + 1 + 2 * lib.sb_sample_adjusted_slices(int(V)) + 1)
 
@@ -316,12 +316,13 @@ def sample_adjusted(out: torch.Tensor, logits: torch.Tensor, temperature: Option
         scratch = torch.zeros(sample_scratch_size(M, V), dtype=torch.int32, device=logits.device)
     wanted.append((scratch, "scratch", i32, None))
     _check(torch.cuda.current_device(), wanted)
+    if M == 0:
+        return
     lib = library()
     check(lib, lib.sb_sample_adjusted(
         _ptr(out), _ptr(logits), _ptr(temperature), _ptr(seeds), _ptr(counters), M, V, scratch.data_ptr(), scratch.numel(), _ptr(history), width,
         _ptr(history_rows), _ptr(prompt_lens), _ptr(lengths), _ptr(penalties), _ptr(bias_starts), _ptr(bias_ids),
-        _ptr(bias_values), _ptr(mask), words, _ptr(mask_rows), _ptr(adjusted), _stream()), "sample_adjusted",
-        kernels=1 if M else 0)
+        _ptr(bias_values), _ptr(mask), words, _ptr(mask_rows), _ptr(adjusted), _stream()), "sample_adjusted")
 
 
 def note_tokens(history: torch.Tensor, ids: torch.Tensor, rows: torch.Tensor, positions: torch.Tensor,
@@ -362,8 +363,10 @@ def copy_pages(k_pools: torch.Tensor, v_pools: torch.Tensor, src: Sequence[int],
         raise KernelError("the pools are empty")
     try:
         a, b = array("i", src), array("i", dst)
-    except (TypeError, OverflowError) as e:
+    except (TypeError, ValueError, OverflowError) as e:
         raise KernelError(f"page numbers must be ints of 32 bits: {e}") from None
+    if len(a) != n or len(b) != n:                          # bytes, of which array() makes ints of four
+        raise KernelError("page numbers must be sequences of ints")
     page = k_pools.stride(1) * k_pools.element_size()
     value_page = v_pools.stride(1) * v_pools.element_size()
     lib = library()
@@ -400,7 +403,8 @@ def attention_shared(out: torch.Tensor, q: torch.Tensor, k_pool: torch.Tensor, v
     Families: group g is the tokens members[group_starts[g]] .. members[group_starts[g + 1] - 1] (int32; a token at most
     once), whose block tables name the same pages for their first shared_lens[g] positions (any number of keys; keys past a
     token's own position are not seen).  A token that shares nothing is a group of its own with length 0.  Tokens in no
-    group are left alone in `out`.  group_starts int32 [groups + 1] starts at 0; empty groups may stand anywhere.
+    group are left alone in `out`.  group_starts int32 [groups + 1] starts at 0; there are at most as many groups as tokens, empty ones
+    anywhere.
 
     Scratch: `part` float32 and `lists` int32 of attention_shared_scratch_size() entries, allocated here if None.
     `status`: int32 word for the bounded waits of the kernel for large families (attention_shared_large), which is not

@@ -34,6 +34,7 @@ from typing import Callable, Iterable, Mapping, Optional, Union
 import numpy as np
 
 MAX_BIASES = 512                 # of one request
+LARGEST = 1e30                   # penalty or bias: with any logit, and counted 10^7 times, it is finite in float32
 
 
 @dataclass(frozen=True)
@@ -52,10 +53,10 @@ class SamplingParams:
         """`vocab`: check token ids, too."""
         if not self.temperature >= 0.0:
             raise ValueError(f"temperature must be >= 0, got {self.temperature}")
-        if not (0.0 < self.repetition_penalty < math.inf):
+        if not 1 / LARGEST <= self.repetition_penalty <= LARGEST:
             raise ValueError(f"repetition_penalty must be positive, got {self.repetition_penalty}")
         for name in ("presence_penalty", "frequency_penalty"):
-            if not math.isfinite(getattr(self, name)):
+            if not abs(getattr(self, name)) <= LARGEST:
                 raise ValueError(f"{name} must be finite, got {getattr(self, name)}")
         if self.logit_bias is not None:
             if len(self.logit_bias) > MAX_BIASES:
@@ -63,7 +64,7 @@ class SamplingParams:
             for t, b in self.logit_bias.items():
                 if vocab is not None and not 0 <= int(t) < vocab:
                     raise ValueError(f"a bias on token {t}, outside the vocabulary of {vocab}")
-                if math.isnan(b) or b == math.inf:
+                if not (abs(b) <= LARGEST or b == -math.inf):
                     raise ValueError(f"a bias of {b} on token {t}")
         if self.allowed is not None and not callable(self.allowed) and vocab is not None:
             if pack_allowed(self.allowed, vocab) is None:

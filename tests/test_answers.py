@@ -270,6 +270,14 @@ def test_params_are_checked():
     assert not SamplingParams(0.7).adjusts and SamplingParams(allowed=[1]).adjusts and SamplingParams(presence_penalty=0.1).penalizes
 
 
+@pytest.mark.parametrize("bad", [dict(repetition_penalty=1e-46), dict(repetition_penalty=1e-40), dict(repetition_penalty=1e39),
+                                 dict(presence_penalty=1e39), dict(frequency_penalty=-1e39), dict(logit_bias={1: 1e39}),
+                                 dict(logit_bias={1: -1e39})], ids=str)
+def test_numbers_that_float32_does_not_hold_are_refused(bad):
+    with pytest.raises(ValueError):
+        SamplingParams(**bad).validate(10)
+
+
 @pytest.mark.parametrize("vocab", [1, 31, 32, 33, 100])
 def test_masks(vocab):
     ids = sorted({0, vocab - 1, vocab // 2})

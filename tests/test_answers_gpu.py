@@ -247,6 +247,26 @@ def test_a_grammar_decides_step_by_step(tmp_path):
         assert len(free.output) == 20
 
 
+def test_penalties_beside_rows_that_were_there_before(tmp_path):
+    """The rows' tokens are kept from the first penalized request on; it may come while others decode, recorded, running ahead,
+    and what the caller does to its biases later changes nothing."""
+    folder = str(make_folder(tmp_path, "A"))
+    kw = dict(dtype="float32", max_batch=4, max_len=128, token_budget=32)
+    eng, bias = Engine(folder, **kw), {7: 2.0, 9: -1.0}
+    first = eng.submit(prompt(20), 40)
+    for _ in range(8):
+        eng.step()
+    assert eng.cache.tokens is None and first.output
+    late = eng.submit_answers(prompt(37, 2), 2, 20, 0.6, 5, repetition_penalty=1.5, frequency_penalty=0.2, logit_bias=bias)
+    bias.clear()
+    eng.run()
+    assert eng.cache.tokens is not None
+    lone = Engine(folder, **kw)
+    assert first.output == lone.generate([prompt(20)], 40)[0]
+    assert [r.output for r in late] == lone.generate([prompt(37, 2)], 20, 0.6, 5, n=2, repetition_penalty=1.5, frequency_penalty=0.2,
+                                                     logit_bias={7: 2.0, 9: -1.0})[0]
+
+
 def test_what_is_refused(tmp_path):
     folder = str(make_folder(tmp_path, "A"))
     eng = Engine(folder, dtype="float32", max_batch=2, max_len=64, token_budget=16, max_queue=3)

@@ -232,6 +232,38 @@ def test_attention_shared_of_more_members_than_the_lists_in_shared_memory_hold()
     check(case, case.run(), case.want())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_attention_shared_of_more_families_than_a_block_has_threads(dtype):
+    case = Case([(16, [1, 2]), (0, [3])] * 150 + [(40, [5] * 9)] + [(0, [7])] * 270, 4, 2, 32, dtype, seed=4).poison()
+    check(case, case.run(), case.want())
+
+
+def test_attention_shared_of_one_family_where_as_many_families_as_members_have_no_place():
+    """512 members of one large family; the lists of 512 families would not fit beside that kernel's tiles."""
+    case = Case([(200, [1, 5] * 256)], 16, 1, 64, torch.bfloat16, seed=6).poison()
+    check(case, case.run(), case.want())
+
+
+def test_attention_shared_on_two_streams_at_once():
+    """Two calls with scratch of their own, large families in both, beside one another again and again."""
+    cases = [Case([(3500, [1, 70, 9] * 8), (64, [40, 3])], 32, 8, 128, torch.bfloat16, seed=s) for s in (1, 2)]
+    outs, calls = [], []
+    for case in cases:
+        want = case.run()
+        sizes = ops.attention_shared_scratch_size(len(case.members), case.heads, case.kv_heads, case.dim, case.page, case.dtype)
+        part, lists = torch.empty(sizes[0], device="cuda"), torch.empty(sizes[1], dtype=torch.int32, device="cuda")
+        outs.append((want, [torch.zeros_like(want) for _ in range(6)]))
+        calls.append((case, part, lists, torch.zeros(1, dtype=torch.int32, device="cuda"), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for i in range(6):
+        for (case, part, lists, word, stream), (_, got) in zip(calls, outs):
+            with torch.cuda.stream(stream):
+                ops.attention_shared(got[i], *case.device, *case.lists, case.heads, case.dim ** -0.5, 0, part, lists, word)
+    torch.cuda.synchronize()
+    for (want, got), (_, _, _, word, _) in zip(outs, calls):
+        assert int(word.item()) == 0 and all(torch.equal(want, x) for x in got)
+
+
 def test_attention_shared_large_families_with_windows():
     case = Case([(3300, [1, 5, 50, 200] * 5), (160, [7] * 7 + [90])], 32, 8, 128, torch.bfloat16, seed=2)
     for window in (3, 150, 2900):
@@ -458,6 +490,51 @@ def test_sample_adjusted_is_sample_where_nothing_is_adjusted():
     assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("V", [7, 1000, 32000, 151936, 151937])
+@pytest.mark.parametrize("spread", [0.0, 1e-3, 2.5, 300.0])
+def test_sample_adjusted_draws_as_sample_at_any_temperature(V, spread):
+    """Which logits' noise is looked at changes no draw: all temperatures, flat and steep rows, the same scratch for both."""
+    g = torch.Generator().manual_seed(V)
+    M = 64
+    logits = (spread * torch.randn(M, V, generator=g)).cuda()
+    logits[5, ::3] = -math.inf
+    logits[6] = -math.inf
+    logits[7, V // 2] = math.inf
+    logits[9, ::2] = math.nan
+    T = torch.exp(6 * torch.rand(M, generator=g) - 3)
+    T[:4] = torch.tensor([0.0, 1e-6, 1e-38, 1e30])
+    kw = dict(temperature=T.cuda(), seeds=ints(torch.randint(-2 ** 31, 2 ** 31, (M,), generator=g).tolist()), counters=ints(range(M)),
+              scratch=torch.zeros(ops.sample_scratch_size(M, V), dtype=torch.int32, device="cuda"))
+    a, b, c = (torch.zeros(M, dtype=torch.int32, device="cuda") for _ in range(3))
+    ops.sample(a, logits, **kw)
+    ops.sample_adjusted(b, logits, **kw)
+    ops.sample(c[:3], logits[:3], **{k: t if k == "scratch" else t[:3] for k, t in kw.items()})
+    assert torch.equal(a, b) and torch.equal(a[:3], c[:3])
+
+
+@pytest.mark.parametrize("W", [4096, 4097, 9001])
+def test_sample_adjusted_long_histories_and_many_biases(W):
+    """Histories beyond what a block holds in registers, hundreds of biases, tokens named again and again by both."""
+    g = torch.Generator().manual_seed(W)
+    M, V = 3, 20000
+    logits = 3 * torch.randn(M, V, generator=g)
+    s = settings(M, V, W, g, masks=False)
+    s["lengths"][:] = torch.tensor([W, W - 3, W // 2], dtype=torch.int32)
+    s["prompt_lens"][:] = torch.tensor([0, W // 2, W], dtype=torch.int32)
+    s["history"] %= 300
+    s["penalties"][:, 2] = 0.001
+    s["bias_starts"] = torch.tensor([0, 700, 700, 1800], dtype=torch.int32)
+    s["bias_ids"] = torch.randint(0, 400, (1800,), generator=g).to(torch.int32)
+    s["bias_values"] = torch.randn(1800, generator=g)
+    tokens, adjusted = sample(logits, s)
+    for m in range(M):
+        want = adjust_64(logits, m, s)
+        # one division or product, two subtractions (9 for a count of 9,000), a sum of up to 30 biases of size 3 in their order: 40 roundings
+        # of values of size 40
+        assert bool(((adjusted[m].double() - want).abs() <= 40 * 2.0 ** -24 * 40).all())
+        assert int(tokens[m]) == int(adjusted[m].argmax())
+
+
 def test_sample_adjusted_ties_nothing_left_and_values_that_are_not_finite():
     V, inf = 300, math.inf
     logits = torch.zeros(5, V)
@@ -524,3 +601,48 @@ def test_sample_adjusted_refusals():
     wide = torch.zeros(1, 262145, device="cuda")
     with pytest.raises(KernelError):
         ops.sample_adjusted(out[:1], wide)
+
+
+def test_bytes_are_no_page_numbers():
+    k, v = (torch.zeros(2, 6, 2, 16, 32, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    for n in (4, 5):
+        with pytest.raises(KernelError):
+            ops.copy_pages(k, v, bytes(n), bytes(n))
+
+
+def test_sample_adjusted_of_no_rows():
+    ops.sample_adjusted(ints([]), torch.zeros(0, 100, device="cuda"))
+    ops.note_tokens(torch.zeros(2, 3, dtype=torch.int32, device="cuda"), ints([]), ints([]), ints([]))
+
+
+@pytest.mark.parametrize("N", [1, 300, 3000])
+@pytest.mark.parametrize("feedback", [True, False])
+def test_note_tokens(N, feedback):
+    g = torch.Generator().manual_seed(N)
+    rows, width = 37, 90
+    place = torch.randperm(rows * width, generator=g)[:N]
+    ids = torch.randint(0, 1000, (N,), generator=g)
+    fed = torch.randint(0, 1000, (50,), generator=g) if feedback else None
+    if feedback:
+        ids[::3] = -1 - torch.randint(0, 50, ids[::3].shape, generator=g)
+    r, p = place // width, place % width
+    want = torch.full((rows, width), 5)
+    want[r, p] = torch.where(ids < 0, fed[(-1 - ids).clamp(0)], ids) if feedback else ids
+    # places outside: nothing is written, and nothing behind the table either
+    outside = [(-1, 0), (rows, 0), (0, -1), (0, width), (2 ** 31 - 1, 2 ** 31 - 1), (-2 ** 31, 5)]
+    for a, b in outside:
+        ids, r, p = (torch.cat([t, torch.tensor([x])]) for t, x in ((ids, 9), (r, a), (p, b)))
+    flat = torch.full((rows * width + 200,), 5, dtype=torch.int32, device="cuda")
+    ops.note_tokens(flat[100:-100].view(rows, width), ints(ids.tolist()), ints(r.tolist()), ints(p.tolist()),
+                    None if fed is None else ints(fed.tolist()))
+    assert torch.equal(flat[100:-100].view(rows, width).cpu().long(), want)
+    assert bool((flat[:100] == 5).all()) and bool((flat[-100:] == 5).all())
+
+
+def test_note_tokens_refusals():
+    h, one = torch.zeros(2, 3, dtype=torch.int32, device="cuda"), ints([1])
+    for bad in ((h.float(), one, one, one), (h[0], one, one, one), (h.t(), one, one, one), (h, one, ints([1, 2]), one),
+                (h, one, one, one.float()), (h.cpu(), one, one, one), (h, one.cpu(), one, one), (h, one, one, one, one.float())):
+        with pytest.raises(KernelError):
+            ops.note_tokens(*bad)
+    assert not bool(h.any())
