@@ -332,6 +332,7 @@ extern "C" int sb_attention_shared(void* out, float* part, long long part_floats
                page_size, table_width, window);
     SB_REQUIRE(N > 0 && M > 0 && M <= N && R > 0 && R <= N && M <= 65535, "attention_shared: %d members of %d tokens in %d groups", M, N, R);
     SB_REQUIRE(dtype == SB_F32 || dtype == SB_BF16, "attention_shared: element type %d", dtype);
+    SB_REQUIRE(scale > 0.f && scale < INFINITY, "attention_shared: a scale of %g", (double)scale);
     const uintptr_t all = reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_pool) |
                           reinterpret_cast<uintptr_t>(v_pool) | reinterpret_cast<uintptr_t>(part) | reinterpret_cast<uintptr_t>(lists);
     SB_REQUIRE(all % 16 == 0, "attention_shared: out, q, the pools and the scratch must start on 16 bytes");

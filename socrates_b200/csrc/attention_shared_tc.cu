@@ -316,6 +316,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constan
             return logical <= ((s.hi - 1) >> bs_log2) ? a.l.block_table[(size_t)unit_table[s.unit] * a.l.table_width + logical] : 0;
         };
         int next = lane < n_ops ? page_of(x0) : 0;
+        int keys = 0, values = 0;                           // tiles whose keys and values were asked for
         for (int t = 0; t < x1 - x0; ++t) {
             const int b = t & 1, y = (next * a.Hkv + kh) * a.BS;
             if (x0 + t + 1 < x1) {
@@ -325,13 +326,18 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constan
             const uint32_t off = b * kv_bytes<D>() + p * PANEL_KV + pg * a.BS * 128;
             if (t >= 2 && !mbar_wait_warp(smem_u32(&s_full[b]), ((t - 2) >> 1) & 1)) { if (lane == 0) give_up(27); break; }
             if (lane == 0) mbar_arrive_expect_tx(smem_u32(&k_full[b]), kv_bytes<D>());
+            keys = t + 1;
             __syncwarp();
             if (lane < n_ops) tma_load_2d(k_s + off, &tma_k, smem_u32(&k_full[b]), p * 64, y);
             if (t >= 2 && !mbar_wait_warp(smem_u32(&v_free[b]), ((t - 2) >> 1) & 1)) { if (lane == 0) give_up(28); break; }
             if (lane == 0) mbar_arrive_expect_tx(smem_u32(&v_full[b]), kv_bytes<D>());
+            values = t + 1;
             __syncwarp();
             if (lane < n_ops) tma_load_2d(v_s + off, &tma_v, smem_u32(&v_full[b]), p * 64, y);
         }
+        // the block outlives its copies, also when a wait gave up (bounded; both buffers' last ones)
+        for (int t = max(0, keys - 2); t < keys; ++t) mbar_wait_warp(smem_u32(&k_full[t & 1]), (t >> 1) & 1);
+        for (int t = max(0, values - 2); t < values; ++t) mbar_wait_warp(smem_u32(&v_full[t & 1]), (t >> 1) & 1);
     } else if (issuer) {
         constexpr uint32_t idesc_qk = make_idesc(KTILE, false);
         const uint64_t dq = make_smem_desc(q_s), dk = make_smem_desc(k_s);
@@ -566,13 +572,6 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap tma_k, const __grid_constan
                 __syncwarp();
                 tcgen05_fence_before();                     // before the next segment's first product writes O
             }
-        }
-    }
-    if (tid == 0 && *((volatile int*)&abort_flag)) {
-        // a wait gave up: let copies in flight land (bounded) before the block exits
-        for (int b = 0; b < 2; ++b) {
-            mbar_wait(smem_u32(&k_full[b]), 0);
-            mbar_wait(smem_u32(&v_full[b]), 0);
         }
     }
     tcgen05_fence_before();

@@ -398,7 +398,7 @@ def attention_shared(out: torch.Tensor, q: torch.Tensor, k_pool: torch.Tensor, v
                      part: Optional[torch.Tensor] = None, lists: Optional[torch.Tensor] = None,
                      status: Optional[torch.Tensor] = None) -> None:
     """Paged attention of single decode tokens whose rows share a prefix: what each shared page holds is read once for all
-    tokens of a family.  Arguments up to `positions` as `attention_decode_mma`; token n is at positions[n] >= 0.
+    tokens of a family.  Arguments up to `positions` as `attention_decode_mma`; token n is at positions[n] >= 0; scale > 0.
 
     Families: group g is the tokens members[group_starts[g]] .. members[group_starts[g + 1] - 1] (int32; a token at most
     once), whose block tables name the same pages for their first shared_lens[g] positions (any number of keys; keys past a

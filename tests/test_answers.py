@@ -330,3 +330,10 @@ def test_c_entries_refuse():
         assert sample(**bad) == 100001, bad
     assert sample(M=0) == 0
     assert lib.sb_note_tokens(p, 0, 4, p, p, p, 1, None, 0, None) == 100001 and lib.sb_note_tokens(p, 2, 4, p, p, p, 0, None, 0, None) == 0
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.125, float("nan"), float("inf")])
+def test_attention_shared_refuses_scales_that_turn_masks_round(scale):
+    lib, p = library(), 0x10000
+    assert lib.sb_attention_shared(p, p, 1 << 40, p, 1 << 30, p, p, p, 10, p, 4, p, p, p, 2, p, p, 1, 2, 4, 2, 64, 16, 0, scale, 1,
+                                   None, None) == 100001
