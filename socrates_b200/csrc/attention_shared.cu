@@ -313,6 +313,11 @@ extern "C" int sb_attention_shared_scratch(int M, int Hq, int Hkv, int D, int pa
 // 1 if a family of n tokens of G query heads a KV head with so many shared keys is a large one, else 0.
 extern "C" int sb_attention_shared_large(int n, int G, int shared) { return n > 0 && G > 0 && sb::tc_family(n, G, shared); }
 
+// 1 if the tensor-core kernels serve bfloat16 calls of so many members, 0 if the one on the CUDA cores does (or none).
+extern "C" int sb_attention_shared_supports(int M, int Hq, int Hkv, int D, int page_size) {
+    return sb::shared_stream_supports(M, M, Hq, Hkv, D, page_size);
+}
+
 // Whether a bfloat16 call launches the kernel for large families too (three kernels instead of two).
 extern "C" int sb_attention_shared_kernels(int M, int R, int Hq, int Hkv, int D, int page_size, int num_pages, int with_status) {
     return Hkv > 0 && with_status && sb::shared_stream_supports(M, R, Hq, Hkv, D, page_size) &&

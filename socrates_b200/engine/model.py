@@ -115,10 +115,10 @@ class Model:
         shares (parts say so through an optional `prefers_shares`; asked once for layers of one shape)."""
         return any(p.prefers_shares(lengths, num_sms) for p in self._key_dealers)
 
-    def prefers_families(self, shared) -> bool:
+    def prefers_families(self, shared, page_size: int) -> bool:
         """Whether a step with families of (rows, shared keys) should read shared keys once (parts say so through an
         optional `prefers_families`)."""
-        return any(p.prefers_families(shared) for p in self._family_readers)
+        return any(p.prefers_families(shared, page_size) for p in self._family_readers)
 
     def has_large_family(self, shared) -> bool:
         return any(p.has_large_family(shared) for p in self._family_readers)

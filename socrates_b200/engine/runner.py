@@ -400,7 +400,7 @@ class ModelRunner:
             n += len(e.tokens)
         members, starts, shared = self.cache.families(rows)
         sizes = [(b - a, k) for a, b, k in zip(starts, starts[1:], shared)]
-        if not self.model.prefers_families(sizes):
+        if not self.model.prefers_families(sizes, self.cache.page_size):
             return None, False
         return ([tokens[i] for i in members], starts, shared), self.model.has_large_family(sizes)
 

@@ -44,6 +44,7 @@ _SIGNATURES = {
     "sb_copy_pages_kernels": [I],
     "sb_attention_shared_scratch": [I, I, I, I, I, I, P, P],
     "sb_attention_shared_large": [I, I, I],
+    "sb_attention_shared_supports": [I, I, I, I, I],
     "sb_attention_shared_kernels": [I, I, I, I, I, I, I, I],
     "sb_attention_shared": [P, P, LL, P, LL, P, P, P, I, P, I, P, P, P, I, P, P, I, I, I, I, I, I, I, F, I, P, P],
     "sb_gemm_simt": [P, P, P, I, I, I, I, I, I, I, I, P],

@@ -78,6 +78,17 @@ SINGLES_APART_FROM = 1024
 SHARED_PAYS_FROM = 36_000_000
 
 
+def reads_shared_keys(members: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int) -> bool:
+    """Whether keys that so many rows share are better read once in this shape: where the tensor-core kernels for that serve it,
+    and where rows one by one have no tensor-core kernel either.  Measured (us a launch; rows one by one / shared keys once; 8 rows
+    behind 8,000 keys, 64 behind 1,024, 64 behind 4,096): 32 heads on 8 of 96 354 / 228, 292 / 161, 953 / 442; 20 on 1 of 128 406 /
+    229, 179 / 108, 573 / 311; but 16 on 4 of 256 394 / 335, 228 / 251, 682 / 638, and 32 on 8 of 128 in pages of 8, which
+    only rows one by one have a tensor-core kernel for, 53 / 266, 163 / 192, 270 / 519."""
+    if ops.attention_shared_supports(members, num_heads, num_kv_heads, head_dim, page_size):
+        return True
+    return head_dim <= 128 and not ops.attention_mma_supports(num_heads, num_kv_heads, head_dim, page_size, True)
+
+
 def balanced_attention(ctx, out, q, k_pool, v_pool, table, num_heads: int, scale: float, window: int) -> None:
     """The step's requests of one token through the equal-shares decode kernel, with scratch of the step."""
     Hkv, D, R = k_pool.shape[1], k_pool.shape[3], ctx.num_seqs
@@ -119,12 +130,13 @@ def paged_attention(ctx, out, q, k_pool, v_pool, table, num_heads: int, scale: f
     `max_len` of the cache alone, so the float32 engine's numbers never depend on the batch.
 
     Where the step says so (`ctx.families`: rows that share a prefix long enough, PAGED_PARTITION "auto", bfloat16, no
-    window), the requests of one token go through `shared_attention` instead.
+    window, a shape of `reads_shared_keys`), the requests of one token go through `shared_attention` instead.
     """
     Hkv, page_size, D = k_pool.shape[1], k_pool.shape[2], k_pool.shape[3]
     N = q.shape[0]
     bf16 = q.dtype == torch.bfloat16
-    shared = bf16 and ctx.families is not None and not window
+    shared = (bf16 and ctx.families is not None and not window
+              and reads_shared_keys(ctx.families[0].numel(), num_heads, Hkv, D, page_size))
     if shared and ctx.all_decode:
         shared_attention(ctx, out, q, k_pool, v_pool, table, num_heads, scale, window)
         return
@@ -266,10 +278,12 @@ class GQAAttention(Part):
         total = sum(lengths) / 64 + N / 2
         return -(-longest // parts) - total / shares >= 8
 
-    def prefers_families(self, shared: Sequence[Tuple[int, int]]) -> bool:
+    def prefers_families(self, shared: Sequence[Tuple[int, int]], page_size: int) -> bool:
         """Whether the requests of one token of a step whose families are `shared`, (rows, shared keys) each, should read shared
         keys once (attention_shared.cu) rather than every row its own way."""
         if self.window or paged_partition() is not None:
+            return False
+        if not reads_shared_keys(sum(n for n, _ in shared), self.Hq, self.Hkv, self.D, page_size):
             return False
         saved = sum((n - 1) * keys for n, keys in shared)
         return saved * self.Hkv * self.D * 4 >= SHARED_PAYS_FROM * (self.Hq // self.Hkv)

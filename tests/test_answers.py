@@ -337,3 +337,17 @@ def test_attention_shared_refuses_scales_that_turn_masks_round(scale):
     lib, p = library(), 0x10000
     assert lib.sb_attention_shared(p, p, 1 << 40, p, 1 << 30, p, p, p, 10, p, 4, p, p, p, 2, p, p, 1, 2, 4, 2, 64, 16, 0, scale, 1,
                                    None, None) == 100001
+
+
+def test_shapes_that_the_engine_reads_shared_keys_with():
+    """The tensor-core kernels' shapes, and head sizes up to 128 that have no tensor-core kernel for rows one by one."""
+    from socrates_b200.kernels import ops
+    from socrates_b200.parts.attention import reads_shared_keys
+    good = dict(members=64, num_heads=32, num_kv_heads=8, head_dim=128, page_size=16)
+    assert ops.attention_shared_supports(**good) and reads_shared_keys(**good)
+    for other in (dict(head_dim=24), dict(head_dim=96), dict(num_heads=136), dict(num_heads=33)):
+        assert not ops.attention_shared_supports(**{**good, **other}) and reads_shared_keys(**{**good, **other}), other
+    for bad in (dict(head_dim=256), dict(page_size=8), dict(members=513)):
+        assert not ops.attention_shared_supports(**{**good, **bad}) and not reads_shared_keys(**{**good, **bad}), bad
+    for wrong in (dict(members=0), dict(num_kv_heads=0)):
+        assert not ops.attention_shared_supports(**{**good, **wrong})

@@ -64,10 +64,10 @@ def test_answers_under_few_pages(tmp_path):
 class Rows:
     """A runner over a random model whose row 0 holds a prompt and rows 1.. are forks of it, all gone on by some tokens."""
 
-    def __init__(self, rows, length, shape=WIDE, dtype=torch.bfloat16, graphs=True, more=3):
+    def __init__(self, rows, length, shape=WIDE, dtype=torch.bfloat16, graphs=True, more=3, page=16):
         config = config_from_dict(shape)
         _, model = build_random_model(config, 7, dtype, torch.device("cuda:0"))
-        self.cache = CacheManager(model.cache_needs(), rows + 2, 2048, 16, 500, dtype, "cuda:0")
+        self.cache = CacheManager(model.cache_needs(), rows + 2, 2048, page, 500, dtype, "cuda:0")
         self.runner = ModelRunner(model, self.cache, dtype, "cuda:0", max_tokens=1600, max_seqs=rows + 2, use_graphs=graphs)
         self.vocab = config.plan().vocab_size
         self.ids = {0: prompt(length, 3, self.vocab)}
@@ -113,6 +113,20 @@ def test_a_step_with_families_gives_the_step_without(always_shared, monkeypatch,
         # bfloat16 activations: a few roundings of 2^-9 of values that add up over four layers, as far as two correct kernels differ
         scale = float(b.abs().max())
         assert float((a - b).abs().max()) <= 2e-2 * scale
+
+
+@pytest.mark.parametrize("shape,page,reads", [(dict(head_dim=96), 16, True), (dict(num_attention_heads=20, num_key_value_heads=1), 16, True),
+                                              (dict(head_dim=256), 16, False), (dict(), 8, False), (dict(), 16, True)], ids=str)
+def test_shapes_whose_shared_keys_are_read_once(always_shared, monkeypatch, shape, page, reads):
+    both = []
+    for least in (1, 1 << 60):
+        monkeypatch.setattr(attention, "SHARED_PAYS_FROM", least)
+        r = Rows(4, 50, {**WIDE, **shape}, page=page)
+        out = [r.feed({i: [11 + i + 7 * k] for i in range(4)}) for k in range(3)]
+        assert any("families" in key for key in r.runner._graphs) == (reads and least == 1)
+        both.append(out)
+    for a, b in zip(*both):                                 # (as far as two correct kernels differ, see above)
+        assert float((a - b).abs().max()) <= 2e-2 * float(b.abs().max())
 
 
 def test_a_recorded_step_follows_its_families(always_shared):
