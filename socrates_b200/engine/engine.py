@@ -23,7 +23,7 @@ import torch
 from ..cache import CacheManager
 from ..config import EngineConfig, load_config
 from ..kernels import require_kernels
-from ..sampling import SamplingParams, pack_allowed
+from ..sampling import AllowedMask, SamplingParams, pack_allowed
 from ..weights import load_weights, random_tensors_on_device
 from .model import Model
 from .runner import Adjust, ModelRunner, SamplingArgs, StepEntry
@@ -157,7 +157,8 @@ class Engine:
                 raise ValueError(f"token id {t} is outside the vocabulary of {vocab}")
         allowed = sampling.get("allowed")
         if allowed is not None and not callable(allowed):
-            sampling["allowed"] = allowed = list(allowed)    # an iterator is walked more than once
+            # an iterator is walked more than once, and what the caller does to theirs later does not matter
+            sampling["allowed"] = allowed = allowed.copy() if isinstance(allowed, AllowedMask) else list(allowed)
         if sampling.get("logit_bias") is not None:
             sampling["logit_bias"] = dict(sampling["logit_bias"])       # what the caller does to theirs later does not matter
         params = [SamplingParams(float(temperature), int(seed) + i, **sampling) for i in range(n)]

@@ -45,8 +45,8 @@ class SamplingParams:
     presence_penalty: float = 0.0        # taken off logits of tokens in the output
     frequency_penalty: float = 0.0       # taken off once for every time a token stands in the output
     logit_bias: Optional[Mapping[int, float]] = None        # token -> what is added to its logit
-    # The tokens that may come next: ids, or a function from the output so far (a list of ids) to ids, to a packed mask
-    # (`pack_allowed`), or to None for all.  A function that allows nothing ends the request.
+    # The tokens that may come next: ids or a packed mask (`pack_allowed`), or a function from the output so far (a list of
+    # ids) to one of these or to None for all.  A function that allows nothing ends the request.
     allowed: Optional[Union[Iterable[int], Callable]] = None
 
     def validate(self, vocab: Optional[int] = None) -> None:
@@ -80,14 +80,22 @@ class SamplingParams:
         return self.penalizes or bool(self.logit_bias) or self.allowed is not None
 
 
-def pack_allowed(allowed, vocab: int) -> Optional[np.ndarray]:
-    """A set of token ids as the mask that the kernel takes: int32 [ceil(vocab / 32)], bit t % 32 of word t // 32.  An array
-    of that type and shape is taken to be one already.  None if nothing is allowed."""
+class AllowedMask(np.ndarray):
+    """A packed mask, int32 [ceil(vocab / 32)]: bit t % 32 of word t // 32 allows token t.  `pack_allowed` makes them, `&` and
+    `|` of two are masks again, and `words.view(AllowedMask)` says that an array is one: nothing else about an array does,
+    as ids may be so many and of that type."""
+
+
+def pack_allowed(allowed, vocab: int) -> Optional[AllowedMask]:
+    """A set of token ids (of any iterable, arrays among them) as the mask that the kernel takes.  An AllowedMask is one already.
+    None if nothing is allowed."""
     words = -(-vocab // 32)
-    if isinstance(allowed, np.ndarray) and allowed.dtype == np.int32 and allowed.shape == (words,):
+    if isinstance(allowed, AllowedMask):
+        if allowed.dtype != np.int32 or allowed.shape != (words,):
+            raise ValueError(f"a mask of {allowed.dtype} {allowed.shape} with a vocabulary of {vocab}")
         tail = vocab % 32
         last = int(allowed[-1]) & ((1 << tail) - 1 if tail else -1)
-        return np.ascontiguousarray(allowed) if last or allowed[:-1].any() else None
+        return allowed if last or allowed[:-1].any() else None
     ids = np.fromiter((int(t) for t in allowed), dtype=np.int64)
     if ids.size == 0:
         return None
@@ -95,7 +103,7 @@ def pack_allowed(allowed, vocab: int) -> Optional[np.ndarray]:
         raise ValueError(f"allowed tokens from {ids.min()} to {ids.max()} with a vocabulary of {vocab}")
     bits = np.zeros(words * 32, dtype=np.uint8)
     bits[ids] = 1
-    return np.packbits(bits, bitorder="little").view("<i4")
+    return np.packbits(bits, bitorder="little").view("<i4").view(AllowedMask)
 
 
-__all__ = ["MAX_BIASES", "SamplingParams", "pack_allowed"]
+__all__ = ["AllowedMask", "MAX_BIASES", "SamplingParams", "pack_allowed"]

@@ -1,0 +1,60 @@
+"""An Engine whose steps run on the host: the scheduler, the cache manager and Engine's own code are the real ones, the model is
+`next_token` of test_scheduler, sampled among the tokens that the step's masks allow."""
+
+from types import SimpleNamespace
+
+import numpy as np
+import torch
+
+from socrates_b200.cache import CacheManager, CacheNeeds, PagedKVSpec
+from socrates_b200.engine.engine import Engine
+from socrates_b200.engine.scheduler import Scheduler
+from test_scheduler import STOP, VOCAB, next_token
+
+
+class HostRunner:
+    """Keeps every row's tokens and answers a step with the first allowed token from `next_token` on."""
+
+    def __init__(self, cache):
+        self.cache, self.tokens, self.sampled, self.steps = cache, {}, [], []
+
+    def step(self, entries, sampling=None, ahead=0, **kw):
+        self.cache.flush()
+        self.steps.append((entries, sampling, kw))
+        before, self.sampled = self.sampled, []
+        args = iter(sampling)
+        for e in entries:
+            held = self.tokens.setdefault(e.row, [])
+            del held[e.start:]
+            held += [before[-1 - t] if t < 0 else t for t in e.tokens]
+            if e.want:
+                mask = getattr(next(args).adjust, "mask", None)
+                t = next_token(held)
+                while mask is not None and not int(mask[t // 32]) >> t % 32 & 1:
+                    t = (t + 1) % VOCAB
+                self.sampled.append(t)
+        return SimpleNamespace(tokens=self.sampled)
+
+    def begin_read(self, count):
+        return list(self.sampled[:count])
+
+    def finish_read(self, handle):
+        return handle
+
+    def check_status(self):
+        pass
+
+
+def host_engine(max_batch=4, max_queue=100, num_pages=64, token_budget=64):
+    """(no forks: rows are fed from their start)"""
+    e = Engine.__new__(Engine)
+    e.model, e.tok, e.max_new_tokens, e.max_len = SimpleNamespace(plan=SimpleNamespace(vocab_size=VOCAB)), None, 8, 256
+    e.cache = CacheManager([CacheNeeds(PagedKVSpec(1, 16, None))], max_batch, 256, 16, num_pages, torch.float32, "cpu")
+    e.runner = HostRunner(e.cache)
+    e.scheduler = Scheduler(e.cache, max_batch, 256, token_budget, max_queue, [STOP])
+    e.run_ahead, e._ahead, e._planned, e.steps, e.ahead_launched, e.ahead_discarded = True, None, None, 0, 0, 0
+    return e
+
+
+def allowed_by(mask, vocab=VOCAB):
+    return [t for t in range(vocab) if int(np.asarray(mask)[t // 32]) >> t % 32 & 1]
