@@ -15,6 +15,7 @@ the tokens of one step.
 from __future__ import annotations
 
 import time
+from dataclasses import replace
 from pathlib import Path
 from typing import List, Optional, Sequence, Union
 
@@ -23,14 +24,12 @@ import torch
 from ..cache import CacheManager
 from ..config import EngineConfig, load_config
 from ..kernels import require_kernels
-from ..sampling import AllowedMask, SamplingParams, pack_allowed
+from ..sampling import SamplingParams, pack_allowed
 from ..weights import load_weights, random_tensors_on_device
 from .model import Model
 from .runner import Adjust, ModelRunner, SamplingArgs, StepEntry
 from .tokenizer import encode_prompt
 from .scheduler import PlannedEntry, QueueFull, Request, Scheduler, StepPlan, TooLong
-
-MOST_ADJUSTED = 262144           # tokens of a vocabulary whose logits can be adjusted (see ops.sample_adjusted)
 
 _DTYPES = {"bfloat16": torch.bfloat16, "bf16": torch.bfloat16, "float32": torch.float32,
            "fp32": torch.float32, torch.bfloat16: torch.bfloat16, torch.float32: torch.float32}
@@ -104,7 +103,7 @@ class Engine:
         if tok is not None:
             stop |= set(getattr(tok, "all_special_ids", ()) or ())
         self.scheduler = Scheduler(self.cache, max_batch, max_len, self.config.token_budget,
-                                   self.config.queue_limit, stop)
+                                   self.config.queue_limit, stop, self.model.plan.vocab_size)
         self.steps = 0
         # run_ahead: while the host waits for a decode step's tokens, the step after it is already
         # on the GPU (see step()); results are the same with and without
@@ -155,19 +154,12 @@ class Engine:
         for t in ids:
             if not 0 <= t < vocab:
                 raise ValueError(f"token id {t} is outside the vocabulary of {vocab}")
-        allowed = sampling.get("allowed")
-        if allowed is not None and not callable(allowed):
-            # an iterator is walked more than once, and what the caller does to theirs later does not matter
-            sampling["allowed"] = allowed = allowed.copy() if isinstance(allowed, AllowedMask) else list(allowed)
-        if sampling.get("logit_bias") is not None:
-            sampling["logit_bias"] = dict(sampling["logit_bias"])       # what the caller does to theirs later does not matter
-        params = [SamplingParams(float(temperature), int(seed) + i, **sampling) for i in range(n)]
-        params[0].validate(vocab)
-        if params[0].adjusts and vocab > MOST_ADJUSTED:
-            raise ValueError(f"logits of {vocab} tokens cannot be adjusted (at most {MOST_ADJUSTED})")
+        first = SamplingParams(float(temperature), int(seed), **sampling)
+        first.validate(vocab)
+        mask = pack_allowed(first.allowed, vocab) if first.allowed is not None and not callable(first.allowed) else None
+        params = [first] + [replace(first, seed=int(seed) + i) for i in range(1, n)]
         if len(self.scheduler.pending) + n > self.scheduler.max_queue:
             raise QueueFull(f"{len(self.scheduler.pending)} requests already waiting, {n} more")
-        mask = pack_allowed(allowed, vocab) if allowed is not None and not callable(allowed) else None
         reqs: List[Request] = []
         for p in params:
             req = Request(ids=ids, max_new_tokens=max_new_tokens or self.max_new_tokens, sampling=p, prompt=text)

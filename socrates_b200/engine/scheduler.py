@@ -39,7 +39,7 @@ from dataclasses import dataclass, field
 from typing import Deque, List, Optional, Sequence
 
 from ..cache.allocator import pages_for
-from ..sampling import SamplingParams
+from ..sampling import MOST_ADJUSTED, SamplingParams, pack_allowed
 
 
 class QueueFull(Exception):
@@ -73,7 +73,7 @@ class Request:
     stream: Optional["queue.Queue"] = None
     # the answers of one prompt, this one among them (see Scheduler); empty: there are no others
     siblings: List["Request"] = field(default_factory=list, repr=False)
-    mask: Optional[object] = field(default=None, repr=False)      # a fixed set of allowed tokens, packed
+    mask: Optional[object] = field(default=None, repr=False)      # a fixed set of allowed tokens, packed at the door
     exhausted: bool = False    # nothing may follow (the request's grammar): the next token drawn ends it
     # scheduler state
     cached: int = 0            # tokens of ids + output that are in the cache
@@ -110,7 +110,8 @@ class StepPlan:
 
 class Scheduler:
     def __init__(self, cache, max_batch: int, max_len: int, token_budget: int, max_queue: int,
-                 stop_ids: Sequence[int] = ()):
+                 stop_ids: Sequence[int] = (), vocab: Optional[int] = None):
+        """`vocab`: of the model, for requests that name tokens (None: the door does not look at those)."""
         if token_budget < max_batch:
             raise ValueError(f"token_budget={token_budget} must cover one token for each of "
                              f"max_batch={max_batch} rows")
@@ -118,6 +119,7 @@ class Scheduler:
         self.max_batch, self.max_len = max_batch, max_len
         self.token_budget, self.max_queue = token_budget, max_queue
         self.stop_ids = frozenset(int(s) for s in stop_ids)
+        self.vocab = vocab
         self.pending: Deque[Request] = deque()
         self.rows: List[Optional[Request]] = [None] * max_batch
         self.n_active = 0
@@ -146,7 +148,13 @@ class Scheduler:
                 need = min(need, pages_for(g.spec.most_keys() + 1, self.cache.page_size) + 1 + g.kept_blocks())
             if need > g.allocator.num_pages:
                 raise TooLong(f"{total} tokens need {need} pages at once; the pool has {g.allocator.num_pages}")
-        req.sampling.validate()
+        p = req.sampling
+        p.validate(self.vocab, packed=req.mask is not None)
+        if self.vocab is not None:
+            if p.adjusts and self.vocab > MOST_ADJUSTED:
+                raise ValueError(f"logits of {self.vocab} tokens cannot be adjusted (at most {MOST_ADJUSTED})")
+            if req.mask is None and p.allowed is not None and not callable(p.allowed):
+                req.mask = pack_allowed(p.allowed, self.vocab)
         self.pending.append(req)
         return req
 

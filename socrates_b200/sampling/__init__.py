@@ -34,6 +34,7 @@ from typing import Callable, Iterable, Mapping, Optional, Union
 import numpy as np
 
 MAX_BIASES = 512                 # of one request
+MOST_ADJUSTED = 262144           # tokens of a vocabulary whose logits can be adjusted (see ops.sample_adjusted)
 LARGEST = 1e30                   # penalty or bias: with any logit, and counted 10^7 times, it is finite in float32
 
 
@@ -49,8 +50,17 @@ class SamplingParams:
     # ids) to one of these or to None for all.  A function that allows nothing ends the request.
     allowed: Optional[Union[Iterable[int], Callable]] = None
 
-    def validate(self, vocab: Optional[int] = None) -> None:
-        """`vocab`: check token ids, too."""
+    def __post_init__(self):
+        # what walks and changes is kept as it is now: iterators are walked more than once, masks are the caller's arrays
+        if isinstance(self.allowed, AllowedMask):
+            object.__setattr__(self, "allowed", self.allowed.copy())
+        elif self.allowed is not None and not callable(self.allowed):
+            object.__setattr__(self, "allowed", list(self.allowed))
+        if self.logit_bias is not None:
+            object.__setattr__(self, "logit_bias", dict(self.logit_bias))
+
+    def validate(self, vocab: Optional[int] = None, packed: bool = False) -> None:
+        """`vocab`: check token ids, too (`packed`: those of a fixed set were, when it was packed)."""
         if not self.temperature >= 0.0:
             raise ValueError(f"temperature must be >= 0, got {self.temperature}")
         if not 1 / LARGEST <= self.repetition_penalty <= LARGEST:
@@ -66,7 +76,7 @@ class SamplingParams:
                     raise ValueError(f"a bias on token {t}, outside the vocabulary of {vocab}")
                 if not (abs(b) <= LARGEST or b == -math.inf):
                     raise ValueError(f"a bias of {b} on token {t}")
-        if self.allowed is not None and not callable(self.allowed) and vocab is not None:
+        if self.allowed is not None and not callable(self.allowed) and vocab is not None and not packed:
             if pack_allowed(self.allowed, vocab) is None:
                 raise ValueError("no token is allowed")
 
@@ -106,4 +116,4 @@ def pack_allowed(allowed, vocab: int) -> Optional[AllowedMask]:
     return np.packbits(bits, bitorder="little").view("<i4").view(AllowedMask)
 
 
-__all__ = ["AllowedMask", "MAX_BIASES", "SamplingParams", "pack_allowed"]
+__all__ = ["AllowedMask", "MAX_BIASES", "MOST_ADJUSTED", "SamplingParams", "pack_allowed"]

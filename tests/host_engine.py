@@ -51,7 +51,7 @@ def host_engine(max_batch=4, max_queue=100, num_pages=64, token_budget=64):
     e.model, e.tok, e.max_new_tokens, e.max_len = SimpleNamespace(plan=SimpleNamespace(vocab_size=VOCAB)), None, 8, 256
     e.cache = CacheManager([CacheNeeds(PagedKVSpec(1, 16, None))], max_batch, 256, 16, num_pages, torch.float32, "cpu")
     e.runner = HostRunner(e.cache)
-    e.scheduler = Scheduler(e.cache, max_batch, 256, token_budget, max_queue, [STOP])
+    e.scheduler = Scheduler(e.cache, max_batch, 256, token_budget, max_queue, [STOP], VOCAB)
     e.run_ahead, e._ahead, e._planned, e.steps, e.ahead_launched, e.ahead_discarded = True, None, None, 0, 0, 0
     return e
 

@@ -4,7 +4,8 @@ import numpy as np
 import pytest
 
 from host_engine import allowed_by, host_engine
-from socrates_b200.sampling import AllowedMask, pack_allowed
+from socrates_b200.engine.scheduler import Request
+from socrates_b200.sampling import AllowedMask, SamplingParams, pack_allowed
 from test_scheduler import STOP, VOCAB
 
 
@@ -40,3 +41,28 @@ def test_answers_hold_allowed_tokens_alone(form):
     for r in reqs:
         assert len(r.output) == 6 and set(r.output) <= {7, 31}
     assert STOP not in (7, 31)
+
+
+@pytest.mark.parametrize("make", [lambda: [7, 31], lambda: iter([7, 31]), lambda: pack_allowed([7, 31], VOCAB), lambda: {7, 31}],
+                         ids=["list", "iterator", "mask", "set"])
+def test_requests_at_the_schedulers_door_keep_to_their_tokens(make):
+    e = host_engine()
+    req = e.scheduler.submit(Request([5, 6], 6, SamplingParams(allowed=make())))
+    e.run()
+    assert len(req.output) == 6 and set(req.output) <= {7, 31}
+
+
+@pytest.mark.parametrize("bad", [dict(allowed=[VOCAB]), dict(allowed=[]), dict(allowed=iter([-1])), dict(logit_bias={VOCAB: 1.0})], ids=str)
+def test_the_schedulers_door_refuses_tokens_that_are_none(bad):
+    e = host_engine()
+    with pytest.raises(ValueError):
+        e.scheduler.submit(Request([5, 6], 6, SamplingParams(**bad)))
+    assert not e.scheduler.has_work()
+
+
+def test_parameters_keep_what_they_were_given():
+    bias, mask, ids = {3: 1.0}, pack_allowed([7], VOCAB), [7]
+    p, q = SamplingParams(logit_bias=bias, allowed=mask), SamplingParams(allowed=ids)
+    bias.clear(), ids.clear()
+    mask[:] = 0
+    assert p.logit_bias == {3: 1.0} and allowed_by(p.allowed) == [7] and q.allowed == [7]
