@@ -132,7 +132,8 @@ class Engine:
         `stream`: the request gets a thread-safe queue `req.stream` that receives each token as
         it is produced and None at the end (the reference's `stream` flag, :132-138).
         `sampling`: the other fields of SamplingParams (repetition_penalty, presence_penalty, frequency_penalty,
-        logit_bias, allowed)."""
+        logit_bias, allowed).  If `allowed` is a function and raises, or names a token outside the vocabulary, the request ends
+        with what it has so far and `req.error` says why."""
         return self.submit_answers(prompt, 1, max_new_tokens, temperature, seed, stream, **sampling)[0]
 
     def submit_answers(self, prompt: Union[str, Sequence[int]], n: int, max_new_tokens: Optional[int] = None,
@@ -193,9 +194,12 @@ class Engine:
             return None
         mask = req.mask
         if callable(p.allowed):
-            allowed = p.allowed(list(req.output))
-            mask = None if allowed is None else pack_allowed(allowed, self.model.plan.vocab_size)
-            req.exhausted = allowed is not None and mask is None
+            try:
+                allowed = p.allowed(list(req.output))
+                mask = None if allowed is None else pack_allowed(allowed, self.model.plan.vocab_size)
+                req.exhausted = allowed is not None and mask is None
+            except Exception as e:          # the caller's: it ends this request, as if nothing might follow, and no other
+                req.error, req.exhausted, mask = e, True, None
         return Adjust(p, row, len(req.ids), length, mask)
 
     def _foresee(self, plan):
@@ -289,14 +293,20 @@ class Engine:
                  temperature: float = 0.0, seed: int = 0, n: int = 1, **sampling):
         """Submit, run, and return the generated ids of each prompt, in order.
         Request i samples with seed + i.  `n` > 1: so many answers a prompt, a list of lists each; answer j of prompt i
-        samples with seed + i * n + j.  `sampling`: as in `submit`."""
+        samples with seed + i * n + j.  `sampling`: as in `submit`; what a grammar raised is raised here, when all are done."""
         if n == 1:
             reqs = [self.submit(p, max_new_tokens, temperature, seed + i, **sampling) for i, p in enumerate(prompts)]
-            self.run()
+            self._finish(reqs)
             return [r.output for r in reqs]
         answers = [self.submit_answers(p, n, max_new_tokens, temperature, seed + i * n, **sampling) for i, p in enumerate(prompts)]
-        self.run()
+        self._finish([r for reqs in answers for r in reqs])
         return [[r.output for r in reqs] for reqs in answers]
+
+    def _finish(self, reqs: Sequence[Request]) -> None:
+        self.run()
+        for r in reqs:
+            if r.error is not None:
+                raise r.error
 
 
 __all__ = ["Engine", "Request", "QueueFull", "TooLong", "build_model", "build_random_model",

@@ -75,6 +75,7 @@ class Request:
     siblings: List["Request"] = field(default_factory=list, repr=False)
     mask: Optional[object] = field(default=None, repr=False)      # a fixed set of allowed tokens, packed at the door
     exhausted: bool = False    # nothing may follow (the request's grammar): the next token drawn ends it
+    error: Optional[Exception] = None      # what the request's grammar raised, which ended the request
     # scheduler state
     cached: int = 0            # tokens of ids + output that are in the cache
     preemptions: int = 0

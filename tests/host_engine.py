@@ -13,10 +13,16 @@ from test_scheduler import STOP, VOCAB, next_token
 
 
 class HostRunner:
-    """Keeps every row's tokens and answers a step with the first allowed token from `next_token` on."""
+    """Keeps the tokens in the rows' pages and answers a step with the first allowed token from `next_token` on."""
 
     def __init__(self, cache):
-        self.cache, self.tokens, self.sampled, self.steps = cache, {}, [], []
+        self.cache, self.sampled, self.steps = cache, [], []
+
+    def place(self, row, pos):
+        g = self.cache.groups[0]
+        page = int(g.host_table[row, pos // 16])
+        assert page
+        return g.k[0, page, 0, pos % 16]
 
     def step(self, entries, sampling=None, ahead=0, **kw):
         self.cache.flush()
@@ -24,10 +30,11 @@ class HostRunner:
         before, self.sampled = self.sampled, []
         args = iter(sampling)
         for e in entries:
-            held = self.tokens.setdefault(e.row, [])
-            del held[e.start:]
-            held += [before[-1 - t] if t < 0 else t for t in e.tokens]
+            end = e.start + len(e.tokens)
+            for pos, t in zip(range(e.start, end), e.tokens):
+                self.place(e.row, pos)[:] = before[-1 - t] if t < 0 else t
             if e.want:
+                held = [int(self.place(e.row, pos)[0]) for pos in range(end)]
                 mask = getattr(next(args).adjust, "mask", None)
                 t = next_token(held)
                 while mask is not None and not int(mask[t // 32]) >> t % 32 & 1:
@@ -46,7 +53,6 @@ class HostRunner:
 
 
 def host_engine(max_batch=4, max_queue=100, num_pages=64, token_budget=64):
-    """(no forks: rows are fed from their start)"""
     e = Engine.__new__(Engine)
     e.model, e.tok, e.max_new_tokens, e.max_len = SimpleNamespace(plan=SimpleNamespace(vocab_size=VOCAB)), None, 8, 256
     e.cache = CacheManager([CacheNeeds(PagedKVSpec(1, 16, None))], max_batch, 256, 16, num_pages, torch.float32, "cpu")
