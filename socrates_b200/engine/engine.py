@@ -159,8 +159,6 @@ class Engine:
         first.validate(vocab)
         mask = pack_allowed(first.allowed, vocab) if first.allowed is not None and not callable(first.allowed) else None
         params = [first] + [replace(first, seed=int(seed) + i) for i in range(1, n)]
-        if len(self.scheduler.pending) + n > self.scheduler.max_queue:
-            raise QueueFull(f"{len(self.scheduler.pending)} requests already waiting, {n} more")
         reqs: List[Request] = []
         for p in params:
             req = Request(ids=ids, max_new_tokens=max_new_tokens or self.max_new_tokens, sampling=p, prompt=text)
@@ -170,8 +168,8 @@ class Engine:
             if stream:
                 import queue
                 req.stream = queue.Queue()
-            reqs.append(self.scheduler.submit(req))
-        return reqs
+            reqs.append(req)
+        return self.scheduler.submit_all(reqs)
 
     # ------------------------------------------------------------------ stepping
     def _launch(self, plan):

@@ -122,6 +122,7 @@ class Scheduler:
         self.stop_ids = frozenset(int(s) for s in stop_ids)
         self.vocab = vocab
         self.pending: Deque[Request] = deque()
+        self._door = threading.Lock()
         self.rows: List[Optional[Request]] = [None] * max_batch
         self.n_active = 0
         self._admissions = 0
@@ -131,8 +132,20 @@ class Scheduler:
 
     # ------------------------------------------------------------------ the door
     def submit(self, req: Request) -> Request:
-        if len(self.pending) >= self.max_queue:
-            raise QueueFull(f"{len(self.pending)} requests already waiting")
+        return self.submit_all([req])[0]
+
+    def submit_all(self, reqs: List[Request]) -> List[Request]:
+        """Queue all of them or, where the queue has no place for so many or one is refused, none; other threads' requests come
+        before or after them."""
+        with self._door:
+            if len(self.pending) + len(reqs) > self.max_queue:
+                raise QueueFull(f"{len(self.pending)} requests already waiting" + (f", {len(reqs)} more" if len(reqs) > 1 else ""))
+            for req in reqs:
+                self._check(req)
+            self.pending.extend(reqs)
+        return reqs
+
+    def _check(self, req: Request) -> None:
         if not req.ids:
             raise ValueError("a prompt needs at least one token")
         if req.max_new_tokens < 1:
@@ -156,8 +169,6 @@ class Scheduler:
                 raise ValueError(f"logits of {self.vocab} tokens cannot be adjusted (at most {MOST_ADJUSTED})")
             if req.mask is None and p.allowed is not None and not callable(p.allowed):
                 req.mask = pack_allowed(p.allowed, self.vocab)
-        self.pending.append(req)
-        return req
 
     @property
     def live(self) -> List[Request]:
