@@ -117,7 +117,8 @@ class Engine:
     def warmup(self) -> None:
         """Record one decode graph per batch width now instead of at the first step of each
         width (the reference warms all its widths in its constructor,
-        model/inference_paged.py:110-130).  Steps that read shared keys once or adjust logits are recorded when they are met."""
+        model/inference_paged.py:110-130).  Steps that read shared keys once and steps that adjust logits have
+        graphs of their own, recorded when they are met; these here stay what they are."""
         t0 = time.perf_counter()
         n = self.runner.warmup(self.max_batch)
         if n:
@@ -180,9 +181,10 @@ class Engine:
         args = [SamplingArgs(t, s, c) for (t, s, c) in self.scheduler.sampling_args(plan)]
         for a, e in zip(args, (e for e in plan.entries if e.samples)):
             a.adjust = self._adjust(e.request, e.row, e.start + e.count)
-        if self.cache.tokens is None and any(e.request.sampling.penalizes for e in plan.entries):
+        note = any(e.request.sampling.penalizes for e in plan.entries)
+        if note:
             self.cache.keep_tokens()        # before the first token of their prompts is computed
-        result = self.runner.step(entries, args)
+        result = self.runner.step(entries, args, note=note)
         return self.runner.begin_read(len(args)) if result.tokens is not None else None
 
     def _adjust(self, req: Request, row: int, length: int) -> Optional[Adjust]:
@@ -253,7 +255,7 @@ class Engine:
             args = [SamplingArgs(req.sampling.temperature, req.sampling.seed, len(req.output) + 1, self._adjust(req, row, start + 1))
                     for (req, row, start) in guess]
             entries = [StepEntry(row, [-1 - j], start, [0]) for j, (_, row, start) in enumerate(guess)]
-            self.runner.step(entries, args, ahead=1)
+            self.runner.step(entries, args, ahead=1, note=any(req.sampling.penalizes for (req, _, _) in guess))
             early = (early_plan, self.runner.begin_read(len(args)), args)
             self.ahead_launched += 1
         # the step's one read-back: sampled tokens and the kernels' status word together

@@ -138,13 +138,14 @@ class _Adjustments:
             event = slot[2] = torch.cuda.Event()
         event.record()
 
-    def of(self, M: int) -> dict:
-        """The keyword arguments of sample_adjusted for M rows."""
+    def of(self, M: int, history: Optional[torch.Tensor]) -> dict:
+        """The keyword arguments of sample_adjusted for M rows; `history`: the rows' tokens, None if no row of them penalizes."""
         at, d = self.at, self.dev
-        return {"history_rows": d[at[0]:at[0] + M], "prompt_lens": d[at[1]:at[1] + M], "lengths": d[at[2]:at[2] + M],
-                "mask_rows": d[at[3]:at[3] + M], "penalties": d[at[4]:at[4] + 3 * M].view(torch.float32).view(M, 3),
-                "bias_starts": d[at[5]:at[5] + M + 1], "bias_ids": d[at[6]:at[7]], "bias_values": d[at[7]:at[8]].view(torch.float32),
-                "mask": self.mask}
+        penalties = {} if history is None else {
+            "history": history, "history_rows": d[at[0]:at[0] + M], "prompt_lens": d[at[1]:at[1] + M], "lengths": d[at[2]:at[2] + M],
+            "penalties": d[at[4]:at[4] + 3 * M].view(torch.float32).view(M, 3)}
+        return {**penalties, "bias_starts": d[at[5]:at[5] + M + 1], "bias_ids": d[at[6]:at[7]],
+                "bias_values": d[at[7]:at[8]].view(torch.float32), "mask": self.mask, "mask_rows": d[at[3]:at[3] + M]}
 
 
 class ModelRunner:
@@ -370,19 +371,24 @@ class ModelRunner:
             raise RuntimeError(f"a tensor-core kernel gave up waiting on its pipeline (code {code}); "
                                f"the step's results are not valid")
 
-    def _run(self, ctx: StepContext, M: int, sample: bool, adjust: bool = False):
+    def _note_tokens(self, N: int) -> None:
+        """Write the step's tokens to the rows' (CacheManager.keep_tokens): before the sampler writes over what ids may stand for,
+        and outside recorded steps, which stay what they are when the first request asks for it."""
+        L, m = self.layout, self.dev_meta
+        ops.note_tokens(self.cache.tokens, m[L.ids:L.ids + N], m[L.rows:L.rows + N], m[L.pos:L.pos + N], self.sampled)
+        self.kernel_launches += 1
+
+    def _run(self, ctx: StepContext, M: int, sample: bool, adjust: bool = False, penalize: bool = False):
         with ops.stream_scope():            # one stream look-up for the step's kernels (also while a graph records)
             logits = self.model.forward(ctx, self.cache)
             tokens = None
-            if self.cache.tokens is not None:       # before the sampler writes over what ids may stand for
-                ops.note_tokens(self.cache.tokens, ctx.token_ids, ctx.token_rows, ctx.positions, self.sampled)
             if sample and M:
                 L, m = self.layout, self.dev_meta
                 tokens = self.sampled[:M]
                 args = (tokens, logits, m[L.temp:L.temp + M].view(torch.float32), m[L.seed:L.seed + M],
                         m[L.counter:L.counter + M], self.sample_scratch)
                 if adjust:
-                    ops.sample_adjusted(*args, history=self.cache.tokens, **self._adjustments.of(M))
+                    ops.sample_adjusted(*args, **self._adjustments.of(M, self.cache.tokens if penalize else None))
                 else:
                     ops.sample(*args)
         return logits, tokens
@@ -415,36 +421,41 @@ class ModelRunner:
     # ------------------------------------------------------------------ the step
     @torch.no_grad()
     def step(self, entries: Sequence[StepEntry],
-             sampling: Optional[Sequence[SamplingArgs]] = None, ahead: int = 0) -> StepResult:
+             sampling: Optional[Sequence[SamplingArgs]] = None, ahead: int = 0, note: bool = True) -> StepResult:
         """Run one batch.  The caller has reserved pages for every entry
         (`cache.reserve(row, start + len(tokens))`) and commits the new lengths after.
         `ahead` = 1: the step is launched before the one before it is committed, so every entry
         starts one past its row's committed length (and may name its token as -1 - j, the j-th
-        token the step before sampled)."""
+        token the step before sampled).
+        `note`: keep the step's tokens if the cache keeps any (False: none of its requests penalizes, now or later)."""
         self.cache.flush()
         families, large = self._families(entries)
         N, M, R, all_decode, max_ctx = self._fill(entries, sampling, ahead, families)
         members = len(families[0]) if families is not None else 0
         sample = sampling is not None
         adjust = sample and any(a.adjust is not None for a in sampling)
+        penalize = adjust and any(a.adjust is not None and a.adjust.params.penalizes for a in sampling)
+        if penalize:
+            self.cache.keep_tokens()
         if adjust:
             if self._adjustments is None:
-                self.cache.keep_tokens()
                 self._adjustments = _Adjustments(self.max_wanted, self.vocab, self.device)
             self._adjustments.fill([a.adjust for a in sampling])
         # decoding rows of very different lengths go through another attention kernel (and a graph of their own)
         share = (all_decode and not members and self.dtype == torch.bfloat16
                  and self.model.prefers_shares([e.start + 1 for e in entries], self.num_sms))
         self.steps_run += 1
+        if note and self.cache.tokens is not None:
+            self._note_tokens(N)
         if self.use_graphs and all_decode and M == N:
             key = (N, sample, share)
-            key += tuple(name for name, on in (("families", members), ("large", large), ("tokens", self.cache.tokens is not None), ("adjust", adjust)) if on)
+            key += tuple(name for name, on in (("families", members), ("large", large), ("adjust", adjust), ("penalize", penalize)) if on)
             if key not in self._graphs and key in self._eager_decode_done:
                 ctx = self._context(N, M, R, True, self.cache.max_len, None, share, members, large)
                 graph = torch.cuda.CUDAGraph()
                 before = Counters.launches
                 with torch.cuda.graph(graph):
-                    logits, tokens = self._run(ctx, M, sample, adjust)
+                    logits, tokens = self._run(ctx, M, sample, adjust, penalize)
                 self._graph_kernels[key] = Counters.launches - before
                 self._graphs[key] = (graph, logits, tokens)
             if key in self._graphs:
@@ -457,7 +468,7 @@ class ModelRunner:
             max_ctx = self.cache.max_len     # the same launch shapes the graph will record
         ctx = self._context(N, M, R, all_decode, max_ctx, entries, share, members, large)
         before = Counters.launches
-        logits, tokens = self._run(ctx, M, sample, adjust)
+        logits, tokens = self._run(ctx, M, sample, adjust, penalize)
         self.kernel_launches += Counters.launches - before
         return StepResult(logits, tokens, N)
 
