@@ -309,11 +309,13 @@ class Scheduler:
         return StepPlan(planned, preempted)
 
     def _sibling(self, req: Request) -> Optional[Request]:
-        """A live answer of the same prompt from whose row `req` can be forked, now or when it has computed the prompt."""
+        """A live answer of the same prompt from whose row `req` can be forked, now or when it has computed the prompt.  (The
+        tokens of a row are kept where its request penalizes: one that does is no fork of one that does not.)"""
         need = len(req.ids) - 1
         if need < 1:
             return None
-        live = [s for s in req.siblings if s is not req and s.row >= 0 and not s.done and not s.cancelled]
+        live = [s for s in req.siblings if s is not req and s.row >= 0 and not s.done and not s.cancelled
+                and (s.sampling.penalizes or not req.sampling.penalizes)]
         for s in live:
             if s.cached >= need and self.cache.can_fork(s.row, need):
                 return s

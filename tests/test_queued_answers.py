@@ -1,4 +1,4 @@
-"""Answers of one prompt are queued all or none, whatever other threads do at the queue's door."""
+"""Answers of one prompt: queued all or none, whatever other threads do at the queue's door, and forked where a fork has what they need."""
 
 import sys
 import threading
@@ -7,6 +7,9 @@ import pytest
 
 from host_engine import host_engine
 from socrates_b200 import QueueFull, TooLong
+from socrates_b200.engine.scheduler import Request
+from socrates_b200.sampling import SamplingParams
+from test_scheduler import expected_output
 
 
 def test_answers_are_queued_all_or_none_beside_other_threads():
@@ -47,3 +50,16 @@ def test_refused_answers_leave_the_queue_alone():
     with pytest.raises(QueueFull):
         e.submit([1, 2])
     assert list(e.scheduler.pending) == reqs and all(r.siblings == reqs for r in reqs)
+
+
+@pytest.mark.parametrize("first,second,forked", [(1.0, 1.0, True), (1.5, 1.5, True), (1.5, 1.0, True), (1.0, 1.5, False)])
+def test_a_row_whose_tokens_are_not_kept_has_no_penalized_fork(first, second, forked):
+    e = host_engine()
+    reqs = [Request([5, 6, 7], 4, SamplingParams(repetition_penalty=r)) for r in (first, second)]
+    for r in reqs:
+        r.siblings = reqs
+        e.scheduler.submit(r)
+    assert e.step() and e.step()
+    assert (e.cache.family[reqs[1].row] > 0) == forked
+    e.run()
+    assert all(r.output == expected_output([5, 6, 7], 4) for r in reqs)
