@@ -321,8 +321,10 @@ class ModelRunner:
     def warmup(self, max_width: int, sample: bool = True) -> int:
         """Record the decode graph of every batch width 1..max_width before serving, as the
         reference does at start-up (model/inference_paged.py:110-130).  The steps run on rows
-        that own no page, so everything they write lands in the null page.  Returns the
-        number of graphs recorded."""
+        that own no page, so everything they write lands in the null page: not beside live ones.
+        Returns the number of graphs recorded."""
+        if any(self.cache.active):
+            raise RuntimeError("steps are warmed before requests are live: they write to the first rows")
         if not self.use_graphs:
             return 0
         made = 0

@@ -68,3 +68,20 @@ def test_bad_grammars_beside_other_requests(tmp_path):
     assert isinstance(beyond.error, ValueError) and len(beyond.output) == 2 and beyond.done and beyond.event.is_set()
     assert free.error is None and free.output == Engine(folder, **kw).generate([prompt(12, 4)], 12)[0]
     assert set(eng.cache.free_pages()) == {eng.num_blocks}
+
+
+def test_a_warm_up_beside_live_requests_is_refused(tmp_path):
+    folder = str(make_folder(tmp_path, "A"))
+    kw = dict(dtype="float32", max_batch=3, max_len=128, token_budget=32)
+    ask = dict(temperature=0.0, repetition_penalty=3.0)
+    want = Engine(folder, **kw).generate([prompt(12)], 16, **ask)[0]
+    eng = Engine(folder, **kw)
+    req = eng.submit(prompt(12), 16, **ask)
+    for _ in range(4):
+        eng.step()
+    with pytest.raises(RuntimeError, match="live"):
+        eng.warmup()
+    eng.run()
+    assert req.output == want
+    eng.warmup()                                            # nobody is live: nothing is disturbed
+    assert eng.generate([prompt(12)], 16, **ask)[0] == want
