@@ -286,10 +286,11 @@ void rows_parts(int M, int Hq, int Hkv, int num_sms, int* NP, int* NS) {
 
 }  // namespace
 
-// Scratch of a call with up to M members in up to M families, in entries: float32, and int32.
-extern "C" int sb_attention_shared_scratch(int M, int Hq, int Hkv, int D, int page_size, int dtype, long long* floats, long long* ints) {
-    SB_REQUIRE(Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && D > 0 && M > 0, "attention_shared: %d members, %d query heads on %d KV heads of %d",
-               M, Hq, Hkv, D);
+// Scratch of a call with up to M members in up to R families (more than M where some are empty), in entries: float32, and int32.
+extern "C" int sb_attention_shared_scratch(int M, int R, int Hq, int Hkv, int D, int page_size, int dtype, long long* floats,
+                                           long long* ints) {
+    SB_REQUIRE(Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && D > 0 && M > 0 && R > 0,
+               "attention_shared: %d members in %d groups, %d query heads on %d KV heads of %d", M, R, Hq, Hkv, D);
     long long most = 0, whole = 1;
     for (int m = 1; m <= M; ++m) {                           // fewer members are cut into more parts
         int NP, NS;
@@ -299,8 +300,8 @@ extern "C" int sb_attention_shared_scratch(int M, int Hq, int Hkv, int D, int pa
     }
     if (dtype == SB_BF16) {
         for (int m = 1; m <= M && sb::shared_stream_supports(m, 1, Hq, Hkv, D, page_size); ++m) {
-            long long f, i;                                  // most families: one a member
-            sb::shared_stream_scratch(m, m, Hq, Hkv, D, page_size, sm_count(), &f, &i);
+            long long f, i;
+            sb::shared_stream_scratch(m, R, Hq, Hkv, D, page_size, sm_count(), &f, &i);
             most = f > most ? f : most;
             whole = i > whole ? i : whole;
         }

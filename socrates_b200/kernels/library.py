@@ -42,7 +42,7 @@ _SIGNATURES = {
     "sb_note_tokens": [P, I, I, P, P, P, I, P, I, P],
     "sb_copy_pages": [P, P, P, P, I, I, I, LL, LL, P],
     "sb_copy_pages_kernels": [I],
-    "sb_attention_shared_scratch": [I, I, I, I, I, I, P, P],
+    "sb_attention_shared_scratch": [I, I, I, I, I, I, I, P, P],
     "sb_attention_shared_large": [I, I, I],
     "sb_attention_shared_supports": [I, I, I, I, I],
     "sb_attention_shared_kernels": [I, I, I, I, I, I, I, I],

@@ -389,13 +389,13 @@ def attention_shared_supports(members: int, num_heads: int, num_kv_heads: int, h
 
 @functools.lru_cache(maxsize=None)
 def attention_shared_scratch_size(members: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int,
-                                  dtype: torch.dtype) -> Tuple[int, int]:
+                                  dtype: torch.dtype, groups: Optional[int] = None) -> Tuple[int, int]:
     """(float32, int32) entries of scratch that `attention_shared` needs for up to so many members, in at most as many
-    groups."""
+    groups (`groups`: or in up to that many, empty ones among them)."""
     floats, ints = ctypes.c_longlong(), ctypes.c_longlong()
     lib = library()
-    check(lib, lib.sb_attention_shared_scratch(members, num_heads, num_kv_heads, head_dim, page_size, _code(dtype),
-                                               ctypes.byref(floats), ctypes.byref(ints)), "attention_shared_scratch_size", kernels=0)
+    check(lib, lib.sb_attention_shared_scratch(members, members if groups is None else groups, num_heads, num_kv_heads, head_dim, page_size,
+                                               _code(dtype), ctypes.byref(floats), ctypes.byref(ints)), "attention_shared_scratch_size", kernels=0)
     return floats.value, ints.value
 
 
@@ -436,7 +436,7 @@ def attention_shared(out: torch.Tensor, q: torch.Tensor, k_pool: torch.Tensor, v
     if M == 0 or R == 0:
         return
     if part is None or lists is None:
-        floats, ints = attention_shared_scratch_size(M, Hq, Hkv, D, BS, q.dtype)
+        floats, ints = attention_shared_scratch_size(M, Hq, Hkv, D, BS, q.dtype, max(M, R))
         part = torch.empty(floats, dtype=torch.float32, device=q.device) if part is None else part
         lists = torch.empty(ints, dtype=torch.int32, device=q.device) if lists is None else lists
     _check(here, ((part, "part", torch.float32, None), (lists, "lists", i32, None)))
