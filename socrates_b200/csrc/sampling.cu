@@ -312,13 +312,12 @@ sample_adjusted_kernel(int* __restrict__ out, const float* __restrict__ logits, 
         });
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         __syncthreads();
-        const float inv_rep = 1.0f / rep;
         auto adjust = [&](int x, bool knows, float value) {
             const int c = atomicExch(&marks[x], 0);          // whoever else names this token gets 0
             if (c == 0) return;
             float l = lg[x];
             const int made = c & MADE;
-            if (c & (PROMPT | MADE)) l *= l > 0.f ? inv_rep : rep;
+            if (c & (PROMPT | MADE)) l = l > 0.f ? l / rep : l * rep;       // one rounding, as the formula has it
             if (made > 0) l = l - frequency * (float)made - presence;
             if (c & BIASED) {
                 if (knows && !(c & TWICE)) l += value;
