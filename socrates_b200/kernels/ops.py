@@ -270,8 +270,8 @@ def sample_adjusted(out: torch.Tensor, logits: torch.Tensor, temperature: Option
 
     out[m] is what `sample` gives for l4 (0 for a row in which nothing is left).  Each of the three parts may be absent:
     * penalties float32 [M, 3] (repetition > 0, presence, frequency) over `history` int32 [rows, width]: row
-      history_rows[m] holds lengths[m] tokens, of which the first prompt_lens[m] are the prompt (int32 [M] each; tokens
-      outside the vocabulary are passed over).  Without penalties the history is not looked at;
+      history_rows[m], a row of it, holds lengths[m] tokens, of which the first prompt_lens[m] are the prompt (int32 [M] each;
+      tokens outside the vocabulary are passed over).  Without penalties the history is not looked at;
     * biases of row m: bias_values[i] (float32) on token bias_ids[i] (int32), i from bias_starts[m] to bias_starts[m + 1] - 1
       (int32 [M + 1]); a token named twice gets both;
     * `mask` int32 [masks, ceil(V / 32)]: bit t % 32 of word t // 32 allows token t; mask_rows[m] (int32 [M]) is the row's
@@ -419,7 +419,8 @@ def attention_shared(out: torch.Tensor, q: torch.Tensor, k_pool: torch.Tensor, v
 
     Read before the kernels wait for the one that precedes them on the stream, so these must be older than that one (a host
     copy, an earlier step): the lists, rows, positions, the block table, and keys and values below each position.  A shared
-    value that only some tokens of a family see (through a window) must be finite: with bfloat16 it meets the others with weight 0."""
+    value that only some tokens of a family see (by their positions or a window) must be finite: the tensor-core kernels weigh it
+    with 0 for the others (the kernel on the CUDA cores does not meet it)."""
     N = q.shape[0]
     if k_pool.dim() != 4:
         raise KernelError(f"k_pool must be [pages, heads, slots, dim], got {tuple(k_pool.shape)}")

@@ -33,3 +33,25 @@ def test_more_groups_than_tokens_are_refused():
     case = Case([(16, [])] * 3 + [(32, [1, 2])], 8, 2, 32, torch.bfloat16)
     with pytest.raises(KernelError):
         case.run()
+
+
+@pytest.mark.parametrize("window", [0, 60])
+@pytest.mark.parametrize("heads,dtype", [((8, 2, 32), torch.float32), ((32, 8, 128), torch.float32), ((12, 4, 96), torch.bfloat16)], ids=str)
+def test_shared_values_that_some_members_see(heads, dtype, window):
+    """The kernel on the CUDA cores keeps a value from those who do not see it, whatever it is: behind a token's position, or before
+    its window.  (The tensor-core kernels weigh it with 0, so there it has to be finite.)"""
+    case = Case([(96, [0, 40, 70])], *heads, dtype, seed=4)
+    a, b, c = case.members
+    row, at = int(case.token_rows[a]), {0: 90, 60: 40}[window]
+    case.positions[a] = 80                                  # sees neither; b and c end at 135 and 165, their windows begin at 76 and 106
+    case.v[int(case.table[row, at // PAGE]), :, at % PAGE] = math.inf
+    got = case.run(window).double().cpu()
+    want = case.want(window)
+    sees = [n for n in case.members if at <= int(case.positions[n]) and (not window or at > int(case.positions[n]) - window)]
+    assert sees == ([b, c] if not window else [a])
+    for n in case.members:
+        if n in sees:
+            assert not bool(torch.isfinite(got[n]).any())
+    others = [n for n in case.members if n not in sees]
+    assert bool(torch.isfinite(got[others]).all())
+    check(case, got[others], want[others])
