@@ -15,6 +15,7 @@ torch.compile(mode="reduce-overhead"), model/inference_paged.py:99-130).
 
 from __future__ import annotations
 
+import gc
 from dataclasses import dataclass, field
 from typing import Dict, List, Optional, Sequence, Tuple
 
@@ -354,12 +355,7 @@ class ModelRunner:
         self._staging[slot][1] = ev
         ctx = self._context(n, n, n, True, self.cache.max_len, None, share)
         self._run(ctx, n, sample)                       # loads every kernel, sizes every buffer
-        graph = torch.cuda.CUDAGraph()
-        before = Counters.launches
-        with torch.cuda.graph(graph):
-            logits, tokens = self._run(ctx, n, sample)
-        self._graph_kernels[key] = Counters.launches - before
-        self._graphs[key] = (graph, logits, tokens)
+        self._record(key, ctx, n, sample)
         self._eager_decode_done.add(key)
         return 1
 
@@ -394,6 +390,21 @@ class ModelRunner:
                 else:
                     ops.sample(*args)
         return logits, tokens
+
+    def _record(self, key: tuple, ctx: StepContext, M: int, *kind) -> None:
+        """Record a step (see _run).  No garbage is collected meanwhile: where an engine of before is among it, the end of its
+        recorded steps would end this recording."""
+        collects = gc.isenabled()
+        gc.disable()
+        try:
+            graph, before = torch.cuda.CUDAGraph(), Counters.launches
+            with torch.cuda.graph(graph):
+                logits, tokens = self._run(ctx, M, *kind)
+        finally:
+            if collects:
+                gc.enable()
+        self._graph_kernels[key] = Counters.launches - before
+        self._graphs[key] = (graph, logits, tokens)
 
     def _families(self, entries: Sequence[StepEntry]):
         """((members, starts, shared lengths) of the entries of one token whose rows share keys, whether a family is large), if
@@ -454,12 +465,7 @@ class ModelRunner:
             key += tuple(name for name, on in (("families", members), ("large", large), ("adjust", adjust), ("penalize", penalize)) if on)
             if key not in self._graphs and key in self._eager_decode_done:
                 ctx = self._context(N, M, R, True, self.cache.max_len, None, share, members, large)
-                graph = torch.cuda.CUDAGraph()
-                before = Counters.launches
-                with torch.cuda.graph(graph):
-                    logits, tokens = self._run(ctx, M, sample, adjust, penalize)
-                self._graph_kernels[key] = Counters.launches - before
-                self._graphs[key] = (graph, logits, tokens)
+                self._record(key, ctx, M, sample, adjust, penalize)
             if key in self._graphs:
                 graph, logits, tokens = self._graphs[key]
                 graph.replay()

@@ -1,5 +1,7 @@
 """Steps with and without adjusted logits side by side: what is recorded stays recorded, and rows keep their own tokens."""
 
+import gc
+
 import pytest
 import torch
 
@@ -85,3 +87,34 @@ def test_a_warm_up_beside_live_requests_is_refused(tmp_path):
     assert req.output == want
     eng.warmup()                                            # nobody is live: nothing is disturbed
     assert eng.generate([prompt(12)], 16, **ask)[0] == want
+
+
+def test_garbage_with_recorded_steps_does_not_end_a_recording(tmp_path, monkeypatch):
+    """What collects garbage while a step is recorded (any allocation may) would reset the recorded steps of an engine that is among
+    it, which is not permitted then."""
+    folder = str(make_folder(tmp_path, "A"))
+    kw = dict(dtype="float32", max_batch=2, max_len=64, token_budget=16)
+    eng = Engine(folder, **kw)
+    want = Engine(folder, **kw).generate([prompt(9)], 12)
+    gc.disable()
+    try:
+        old = Engine(folder, **kw)
+        assert old.generate([prompt(9)], 12) == want and old.runner._graphs
+        old.itself = old
+        del old
+        forward, recorded = type(eng.model).forward, []
+
+        def collecting(self, ctx, cache):
+            if torch.cuda.is_current_stream_capturing():
+                recorded.append(1)
+                if gc.isenabled():
+                    gc.collect()
+            return forward(self, ctx, cache)
+
+        monkeypatch.setattr(type(eng.model), "forward", collecting)
+        gc.enable()
+        gc.freeze()                                         # young garbage waits for the collection above
+        gc.unfreeze()
+        assert eng.generate([prompt(9)], 12) == want and recorded and gc.isenabled()
+    finally:
+        gc.enable()
