@@ -6,8 +6,8 @@
 //   m = max(m_S, m_T),  l = e^{m_S - m} l_S + e^{m_T - m} l_T,  o = (e^{m_S - m} o_S + e^{m_T - m} o_T) / l,
 // so the family's query heads (tokens x G rows) meet S as the rows of one tile and every token meets its own T_n as G rows.
 //
-// This file's kernel runs on the CUDA cores in float32: the 32-bit engine, and in bfloat16 the shapes that the tensor-core
-// kernels do not take.  A block serves 16 rows of one KV head (of a family: any 16 of its tokens x G rows; of one token: its
+// This file's kernel runs on the CUDA cores in float32: calls in float32 (the 32-bit engine makes none, as its numbers do not
+// depend on the batch), and in bfloat16 the shapes that the tensor-core kernels do not take.  A block serves 16 rows of one KV head (of a family: any 16 of its tokens x G rows; of one token: its
 // G rows) and one part of their keys; parts are joined by a second kernel.
 #include <math.h>
 

@@ -497,7 +497,9 @@ int stream_smem(int M, int R, int G, int D) {
     return (STAGES * 2 * KT * D + STAGES * RQ * D) * 2 + PAGE_SLOTS * TILE_PAGES * 4 + list_ints(M, R, most_units(M, R, G)) * 4;
 }
 
-// Blocks of a KV head: as many as the GPU holds at once (two an SM, or one beside long lists).
+// Blocks of a KV head: as many as the GPU holds at once (two an SM, or one beside long lists: from 83 members in as many groups on
+// at 4 query heads a KV head of 128, from 77 at 8.  One family behind 4,096 keys with up to 1,024 of their own, us a call in a
+// graph: 32 query heads, 82 members 82, 84 members 110; 64 query heads, 76 members 85, 78 members 120).
 int blocks_of(int M, int R, int Hq, int Hkv, int D, int num_sms) {
     const int w = num_sms * (stream_smem(M, R, Hq / Hkv, D) <= TWO_AN_SM ? 2 : 1) / Hkv;
     return w < 1 ? 1 : w;

@@ -176,7 +176,7 @@ constexpr int SLICE = 8192;          // logits of a block at most, held in share
 // most l can exceed it only where N - 1/2 <= 2^23 e^(l / T - F), a bound on the hash that a thread takes once, with its
 // largest logit.  The others are not looked at.
 // 64 rows of 151,936 logits, half of them drawn, tokens of up to 4,096 and 40 biases a row: 60 us a logit at a time with tables for
-// counts and biases, 42 with 16 logits a thread in registers, 29 so (22 if none is drawn, 14 if nothing is adjusted either).
+// counts and biases, 42 with 16 logits a thread in registers, 30 so (22 if none is drawn, 14 if nothing is adjusted either).
 __global__ void __launch_bounds__(512, 3)
 sample_adjusted_kernel(int* __restrict__ out, const float* __restrict__ logits, const float* __restrict__ temperature,
                        const uint32_t* __restrict__ seeds, const uint32_t* __restrict__ counters, int V, int per,

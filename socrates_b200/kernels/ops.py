@@ -383,7 +383,7 @@ def attention_shared_large(tokens: int, group: int, shared: int) -> bool:
 @functools.lru_cache(maxsize=None)
 def attention_shared_supports(members: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int) -> bool:
     """Whether the tensor-core kernels serve `attention_shared` with so many members in bfloat16; other shapes go through
-    the kernel of the 32-bit engine (head sizes that are multiples of 16, up to 256)."""
+    the kernel on the CUDA cores, as float32 does (head sizes that are multiples of 16, up to 256)."""
     return bool(library().sb_attention_shared_supports(members, num_heads, num_kv_heads, head_dim, page_size))
 
 

@@ -74,7 +74,9 @@ SINGLES_APART_FROM = 1024
 # behind 1,024 (130) 2.96 / 3.25, 24 behind 2,048 (193) 3.60 / 3.20, 8 behind 8,000 (229) 3.42 / 3.05, 64 behind 1,024 (264) 4.45 / 4.07,
 # 32 behind 4,096 (520) 5.44 / 3.74, 64 behind 8,000 (2,064) 14.22 / 4.94.  By the heads, because their rows are what the shared keys
 # are read for: launches of 64 query heads on 8 KV heads (us, the faster of the other kernels / this) 4 rows behind 8,192 (101)
-# 24 / 32, 8 behind 4,096 (117) 26 / 32, 8 behind 8,192 (235) 44 / 37, 64 behind 1,024 (264) 49 / 44.
+# 24 / 32, 8 behind 4,096 (117) 26 / 32, 8 behind 8,192 (235) 44 / 37, 16 behind 4,096 (252) 44 / 36, 64 behind 1,024 (264)
+# 49 / 44.  The bound was fitted at 4 heads; at 8 it is 288 MB, past where launches are even (about 200), so that some steps that
+# would gain up to a fifth of their attention read every row its own way.
 SHARED_PAYS_FROM = 36_000_000
 
 
