@@ -370,16 +370,16 @@ class ModelRunner:
                                f"the step's results are not valid")
 
     def _note_tokens(self, N: int) -> None:
-        """Write the step's tokens to the rows' (CacheManager.keep_tokens): before the sampler writes over what ids may stand for,
-        and outside recorded steps, which stay what they are when the first request asks for it."""
+        """Write the step's tokens to the rows' (CacheManager.keep_tokens), before the sampler writes over what ids may stand for."""
         L, m = self.layout, self.dev_meta
         ops.note_tokens(self.cache.tokens, m[L.ids:L.ids + N], m[L.rows:L.rows + N], m[L.pos:L.pos + N], self.sampled)
-        self.kernel_launches += 1
 
     def _run(self, ctx: StepContext, M: int, sample: bool, adjust: bool = False, penalize: bool = False):
         with ops.stream_scope():            # one stream look-up for the step's kernels (also while a graph records)
             logits = self.model.forward(ctx, self.cache)
             tokens = None
+            if penalize:
+                self._note_tokens(ctx.num_tokens)
             if sample and M:
                 L, m = self.layout, self.dev_meta
                 tokens = self.sampled[:M]
@@ -440,7 +440,8 @@ class ModelRunner:
         `ahead` = 1: the step is launched before the one before it is committed, so every entry
         starts one past its row's committed length (and may name its token as -1 - j, the j-th
         token the step before sampled).
-        `note`: keep the step's tokens if the cache keeps any (False: none of its requests penalizes, now or later)."""
+        `note`: keep the step's tokens if the cache keeps any (False: none of its requests penalizes, now or later; a step that
+        samples under penalties keeps them in any case)."""
         self.cache.flush()
         families, large = self._families(entries)
         N, M, R, all_decode, max_ctx = self._fill(entries, sampling, ahead, families)
@@ -458,8 +459,9 @@ class ModelRunner:
         share = (all_decode and not members and self.dtype == torch.bfloat16
                  and self.model.prefers_shares([e.start + 1 for e in entries], self.num_sms))
         self.steps_run += 1
-        if note and self.cache.tokens is not None:
-            self._note_tokens(N)
+        if note and not penalize and self.cache.tokens is not None:
+            self._note_tokens(N)            # outside recorded steps, which stay what they are when the first request penalizes
+            self.kernel_launches += 1
         if self.use_graphs and all_decode and M == N:
             key = (N, sample, share)
             key += tuple(name for name, on in (("families", members), ("large", large), ("adjust", adjust), ("penalize", penalize)) if on)
